@@ -50,6 +50,7 @@ typedef struct s3dsp_fc_tables s3dsp_fc_tables;
 typedef struct s3dsp_mesh s3dsp_mesh;
 typedef struct s3dsp_gguf s3dsp_gguf;
 typedef struct s3dsp_shard s3dsp_shard;
+typedef struct s3dsp_attn_plan s3dsp_attn_plan;
 
 /* element types */
 #define S3DSP_F32 UINT32_C(0)
@@ -93,6 +94,15 @@ typedef struct s3dsp_shard s3dsp_shard;
                                           one CTA per 128-row tile; same results, slower on B200 today */
 #define S3DSP_CONV_HALO UINT32_C(256)    /* BF16: force the per-tile input halo kernel (one source, cin <= 256,
                                             cout <= 128, kvol <= 27; other layers ignore the flag) */
+
+/* rotation and per-head norm flags (s3dsp_rope, s3dsp_qk_norm_rope) */
+#define S3DSP_ROPE_HALF UINT32_C(1)       /* pair j of a head is (j, j + d/2); without it (2j, 2j + 1) */
+#define S3DSP_ROPE_INVERSE UINT32_C(2)    /* turn by the negative angles (undoes the rotation) */
+#define S3DSP_QK_GAMMA_SHARED UINT32_C(4) /* one weight row [d] for every head instead of [heads, d] */
+
+/* rows of the blocks that s3dsp_attn_plan_create cuts sequences into */
+#define S3DSP_ATTN_Q_ROWS 128
+#define S3DSP_ATTN_K_ROWS 64
 
 /* context flags */
 #define S3DSP_CONTEXT_DEFERRED_CHECKS UINT32_C(1) /* device-detected input errors are reported by
@@ -371,6 +381,93 @@ S3DSP_API s3d_status s3dsp_window_attention(s3dsp_context *ctx, const float *qkv
                                             int32_t heads, const int32_t *d_windows, int64_t n_windows,
                                             const int32_t *d_scatter, float *out, char *error,
                                             uint64_t error_capacity);
+
+/* ---------------------------------------------------------------------------
+ * Attention over voxel tokens: the transformer between the SLat generator's
+ * sparse stages (its blocks run on the coarse rows of s3dsp_slat_tables; a
+ * batch of objects is a ragged batch of sequences, one after another). Rows
+ * are [n, heads * d] with a row stride in elements, head h at columns
+ * h*d .. h*d+d-1, so q, k and v may be slices of one fused projection. Head
+ * groups: query head h reads key head h / (heads / kv_heads). No counterpart
+ * in the reference's sparse path (its dense transformer is GGML's).
+ * ------------------------------------------------------------------------- */
+/* y = x with every head turned by the row's position. A head's d/2 pairs are
+ * dealt to the axes in order: axis_pairs[0] (host int32 [axes], axes <= 4)
+ * pairs turn with position column 0, the next axis_pairs[1] with column 1, ...;
+ * the rest stay. Pair i of an axis with p pairs turns by pos * theta^(-i/p);
+ * (a, b) -> (a cos - b sin, a sin + b cos). Angles are reduced to a turn in f64
+ * (within |pos| 2^-50 for every int32 position), their remainder is f32. d_pos: device int32 rows with a stride of
+ * pos_stride elements; voxel rows (batch, x, y, z) are d_coords + 1 with
+ * stride 4. d a multiple of 8 up to 256; any strides >= heads * d and element
+ * alignment (16-byte aligned rows are read and written 16 bytes at a time).
+ * y may be x with the same stride and type, and must not overlap it
+ * otherwise. Arithmetic in f32, rounded once to y_dtype. flags:
+ * S3DSP_ROPE_HALF, S3DSP_ROPE_INVERSE (the rotation's transpose: also what
+ * maps a gradient of y to one of x). */
+S3DSP_API s3d_status s3dsp_rope(s3dsp_context *ctx, const void *x, uint32_t x_dtype, int64_t n, int64_t x_stride,
+                                int32_t heads, int32_t d, const int32_t *d_pos, int64_t pos_stride, int32_t axes,
+                                const int32_t *axis_pairs, double theta, uint32_t flags, void *y, uint32_t y_dtype,
+                                int64_t y_stride, char *error, uint64_t error_capacity);
+/* The norms of queries and keys and their rotation in one pass: per row and
+ * head x / sqrt(mean(x^2) + eps) * gamma, then s3dsp_rope's rotation (axes 0:
+ * none). q_gamma f32 [heads, d], k_gamma f32 [kv_heads, d] (both [d] with
+ * S3DSP_QK_GAMMA_SHARED; NULL: ones). k NULL (kv_heads 0, k_out NULL)
+ * normalises q alone. Strides, alignment, in-place use and rounding as
+ * s3dsp_rope. flags: S3DSP_ROPE_HALF, S3DSP_QK_GAMMA_SHARED. */
+S3DSP_API s3d_status s3dsp_qk_norm_rope(s3dsp_context *ctx, const void *q, int64_t q_stride, int32_t heads,
+                                        const float *q_gamma, const void *k, int64_t k_stride, int32_t kv_heads,
+                                        const float *k_gamma, uint32_t x_dtype, int64_t n, int32_t d, float eps,
+                                        const int32_t *d_pos, int64_t pos_stride, int32_t axes,
+                                        const int32_t *axis_pairs, double theta, uint32_t flags, void *q_out,
+                                        int64_t q_out_stride, void *k_out, int64_t k_out_stride, uint32_t y_dtype,
+                                        char *error, uint64_t error_capacity);
+/* The block tables of a ragged batch: sequence s has query rows
+ * [h_q_offsets[s], h_q_offsets[s+1]) and key rows [h_k_offsets[s],
+ * h_k_offsets[s+1]) (host int64 [n_seq + 1], non-decreasing, ends below
+ * 2^31 - 255; h_k_offsets NULL: the key rows are the query rows; empty
+ * sequences are fine). Every sequence is cut into query blocks of
+ * S3DSP_ATTN_Q_ROWS rows and key blocks of S3DSP_ATTN_K_ROWS, counted from
+ * its own first row, the last ones shorter. Made from host memory on the
+ * context's stream (not inside a stream capture; calls that use the plan may
+ * be captured). Freed by s3dsp_attn_plan_free. */
+S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context *ctx, const int64_t *h_q_offsets,
+                                            const int64_t *h_k_offsets, int64_t n_seq, s3dsp_attn_plan **out,
+                                            char *error, uint64_t error_capacity);
+S3DSP_API void s3dsp_attn_plan_free(s3dsp_context *ctx, s3dsp_attn_plan *plan);
+/* Rows that the plan spans (its last offsets), its query and key blocks and
+ * the most key blocks of one sequence; any pointer may be NULL. */
+S3DSP_API s3d_status s3dsp_attn_plan_info(const s3dsp_attn_plan *plan, int64_t *n_q, int64_t *n_k,
+                                          int64_t *q_blocks, int64_t *k_blocks, int64_t *max_k_blocks);
+/* For every query block and head, the `top` (1 .. 1024) key blocks of its
+ * sequence with the largest score <mean of the block's q rows, mean of the key
+ * block's k rows>: d_sel int32 [q blocks, heads, top], ascending indices
+ * counted from the sequence's first key block, -1 behind them when the
+ * sequence has fewer. Ties go to the lowest index, a NaN score is the lowest.
+ * Means and scores are f64, so a list does not depend on the order of sums.
+ * keep_local != 0 (self attention plans only): the key blocks of the query
+ * block's own rows come first. d a multiple of 8 up to 256, any strides; a
+ * sequence has at most about 24,000 key blocks. */
+S3DSP_API s3d_status s3dsp_block_select(s3dsp_context *ctx, const s3dsp_attn_plan *plan, const void *q,
+                                        int64_t q_stride, int32_t heads, const void *k, int64_t k_stride,
+                                        int32_t kv_heads, uint32_t dtype, int32_t d, int32_t top,
+                                        int32_t keep_local, int32_t *d_sel, char *error, uint64_t error_capacity);
+/* out = softmax(scale * q k^T over the listed key blocks' rows) v, per row and
+ * head; d_sel NULL: over all key rows of the row's sequence. d_sel int32 [q
+ * blocks, heads, top] (top <= 1024) as s3dsp_block_select writes it: entries
+ * below 0 are skipped, a block listed twice counts twice, an entry past the
+ * sequence's key blocks is skipped and reported by the next status check. A
+ * row with nothing to attend to (no listed block, no key row, or every score
+ * -inf) gets zeros. Rows of out outside the plan's sequences are left as they
+ * are. dtype S3DSP_BF16 or S3DSP_F16 for q, k, v and out; scores, softmax
+ * statistics and sums in f32, the weights exp(s - max) rounded to dtype for
+ * the product with v (tcgen05 MMAs). d 64 or 128; scale > 0 and finite;
+ * pointers 16-byte aligned, row strides multiples of 8 elements. out must not
+ * overlap the inputs. */
+S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context *ctx, const s3dsp_attn_plan *plan, const void *q,
+                                           int64_t q_stride, int32_t heads, const void *k, int64_t k_stride,
+                                           const void *v, int64_t v_stride, int32_t kv_heads, uint32_t dtype,
+                                           int32_t d, float scale, const int32_t *d_sel, int32_t top, void *out,
+                                           int64_t out_stride, char *error, uint64_t error_capacity);
 
 /* ---------------------------------------------------------------------------
  * FlexiCubes extraction at resolution 256 (extract_object_mesh,

@@ -1,0 +1,500 @@
+// Block attention: out = softmax(scale q k^T) v of each query row over the
+// rows of its listed key blocks (64 rows each), or over its whole sequence.
+//
+// One CTA per (query block of 128 rows, head). The row maximum and sum run
+// along with the blocks (online softmax), so scores never leave the SM:
+//
+//   producer warp   TMA: the Q tile once, then the K and V tiles of the listed blocks into rings
+//   MMA warp        S = Q K^T (tcgen05, f32 in TMEM), then O += P V with P read from TMEM
+//   softmax warps   one thread per query row: S from TMEM, running maximum, p = 2^(c s - c m),
+//                   running sum, P back into S's columns
+//
+// S is double-buffered: the next block's scores are computed while this
+// block's softmax runs, and P(j) V(j) while softmax(j + 1) runs. A buffer is
+// written by Q K^T(j + 2) only after P(j) V(j), its last reader, has completed.
+//
+// The accumulator is rescaled only when a row's maximum has grown by more than
+// kSlack (in powers of two) over the one in use: the softmax is the same for
+// any reference near the maximum, p <= 2^kSlack stays well inside f32 and f16,
+// and a rescale is a round trip of O through TMEM. P is rounded to the input
+// type (8 or 11 bits, as v has); its sum is taken before that, in f32.
+//
+// Rows past the block's keys: their scores are replaced by -inf (so p is 0)
+// and their V rows by zeros in shared memory, whatever they hold.
+#include <cmath>
+
+#include "tc_common.cuh"
+
+using namespace s3dsp;
+using namespace s3dsp::tc;
+
+namespace {
+
+constexpr int kQ = kAttnQRows, kK = kAttnKRows;
+constexpr int kQPanel = kQ * 128, kKPanel = kK * 128;  // bytes of 64 columns of a Q / K / V tile
+constexpr float kSlack = 8.f;
+
+struct AttnParams {
+    const int4* q_blocks;
+    const int32_t* sel;  // [n_qb][heads][top], or nullptr
+    int top, heads, per_kv;
+    float c;  // scale * log2(e)
+    void* out;
+    int64_t out_stride;
+    uint32_t* status;
+};
+
+template <int D>
+struct Cfg {
+    static constexpr int kPanels = D / 64;
+    static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;  // ring depths: two CTAs per SM
+    static constexpr int kThreads = 128 + 64;
+    static constexpr int kTmemCols = 256;  // S0 64 | S1 64 | O D
+    static constexpr int kOCol = 128;
+    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 2 + 2 + 1 + 1;
+    static constexpr size_t kTiles = (size_t)kPanels * kQPanel + (size_t)(kKS + kVS) * kPanels * kKPanel;
+    static constexpr size_t smem(int list) { return 1024 + kTiles + kBars * 8 + 16 + (size_t)list * 4; }
+};
+
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// D (f32, TMEM) += A (16-bit, TMEM) * B (shared memory)
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// 16-bit operand whose N (or M) index is contiguous: 128-byte rows of 64
+// columns, one row per K index, 128-byte swizzle; 8-row groups 1,024 bytes
+// apart along K, 64-column panels kKPanel bytes apart along N.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kKPanel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+#define S3DSP_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), \
+                       "=r"(v[o + 6]), "=r"(v[o + 7])
+#define S3DSP_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), \
+                       "r"(v[o + 6]), "r"(v[o + 7])
+#define S3DSP_RW8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), \
+                        "+r"(v[o + 6]), "+r"(v[o + 7])
+// 32 columns of this thread's TMEM lane (no wait)
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : S3DSP_R8(v, 0), S3DSP_R8(v, 8), S3DSP_R8(v, 16), S3DSP_R8(v, 24)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::S3DSP_I8(v, 0),
+        S3DSP_I8(v, 8), S3DSP_I8(v, 16), S3DSP_I8(v, 24), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::S3DSP_I8(
+            v, 0),
+        S3DSP_I8(v, 8), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// values loaded by tmem_ld32, usable only from here on: the compiler sees them
+// change after the wait, so no use moves before it
+__device__ __forceinline__ void tmem_settle(uint32_t (&v)[32]) {
+    asm volatile("" : S3DSP_RW8(v, 0), S3DSP_RW8(v, 8), S3DSP_RW8(v, 16), S3DSP_RW8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// the larger of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float exp2_hw(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// (lo, hi) as two 16-bit floats of one register
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (kF16)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int D, bool kF16>
+__global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
+    block_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                           const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
+    using C = Cfg<D>;
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t* sm = raw + (base - smem_u32(raw));
+    const uint32_t sQ = base, sK = sQ + C::kPanels * kQPanel, sV = sK + C::kKS * C::kPanels * kKPanel;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles);
+    const uint32_t b0 = smem_u32(bars);
+    const uint32_t q_full = b0, k_full = b0 + 8, k_empty = k_full + 8 * C::kKS, v_full = k_empty + 8 * C::kKS,
+                   v_empty = v_full + 8 * C::kVS, s_full = v_empty + 8 * C::kVS, p_full = s_full + 16,
+                   o_done = p_full + 16, drained = o_done + 8;
+    volatile int* abort_flag = reinterpret_cast<int*>(bars + C::kBars);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + C::kBars) + 1;
+    volatile int* n_listed = reinterpret_cast<int*>(bars + C::kBars) + 2;
+    volatile int* drain_flag = reinterpret_cast<int*>(bars + C::kBars) + 3;
+    int* list = reinterpret_cast<int*>(bars + C::kBars) + 4;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kProdWarp = 4, kMmaWarp = 5;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < C::kKS; ++s) mbar_init(k_full + 8 * s, 1), mbar_init(k_empty + 8 * s, 1);
+        for (int s = 0; s < C::kVS; ++s) mbar_init(v_full + 8 * s, 1), mbar_init(v_empty + 8 * s, 1);
+        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, kQ);
+        mbar_init(o_done, 1);
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        *drain_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"((uint32_t)C::kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    const int h = blockIdx.y;
+    const int4 qb = p.q_blocks[blockIdx.x];
+    const int q_row0 = qb.x, q_rows = qb.y & kAttnRowsMask, k_row0 = qb.z, k_rows = qb.w;
+    const int nkb = (k_rows + kK - 1) / kK;
+    if (warp == 0) {
+        // the listed blocks that exist, in list order
+        int n = nkb;
+        if (p.sel) {
+            const int32_t* row = p.sel + ((int64_t)blockIdx.x * p.heads + h) * p.top;
+            n = 0;
+            for (int i0 = 0; i0 < p.top; i0 += 32) {
+                const int e = i0 + lane < p.top ? __ldg(row + i0 + lane) : -1;
+                if (e >= nkb) atomicOr(p.status, kErrRowRange);
+                const unsigned m = __ballot_sync(0xffffffffu, e >= 0 && e < nkb);
+                if (e >= 0 && e < nkb) list[n + __popc(m & ((1u << lane) - 1u))] = e;
+                n += __popc(m);
+            }
+        }
+        if (lane == 0) *n_listed = n;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();
+    const uint32_t tmem = *tmem_holder;
+    const int n = *n_listed;
+    auto block_of = [&](int j) { return p.sel ? list[j] : j; };
+    auto rows_of = [&](int blk) { return min(kK, k_rows - blk * kK); };
+
+    if (warp == kProdWarp) {
+        // ================= TMA producer =================
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
+            const int qc = h * D, kc = (h / p.per_kv) * D;
+            mbar_arrive_tx(q_full, C::kPanels * kQPanel);
+            for (int i = 0; i < C::kPanels; ++i) tma_load_2d(sQ + i * kQPanel, &qmap, qc + 64 * i, q_row0, q_full);
+            int issued_k = 0, issued_v = 0;
+            bool ok = true;
+            for (int j = 0; j < n && ok; ++j) {
+                const int y = k_row0 + block_of(j) * kK;
+                const int s = j % C::kKS, t = j % C::kVS;
+                ok = mbar_wait(k_empty + 8 * s, ((j / C::kKS) & 1) ^ 1, abort_flag, p.status);
+                if (!ok) break;
+                mbar_arrive_tx(k_full + 8 * s, kTileBytes);
+                for (int i = 0; i < C::kPanels; ++i)
+                    tma_load_2d(sK + s * kTileBytes + i * kKPanel, &kmap, kc + 64 * i, y, k_full + 8 * s);
+                ++issued_k;
+                ok = mbar_wait(v_empty + 8 * t, ((j / C::kVS) & 1) ^ 1, abort_flag, p.status);
+                if (!ok) break;
+                mbar_arrive_tx(v_full + 8 * t, kTileBytes);
+                for (int i = 0; i < C::kPanels; ++i)
+                    tma_load_2d(sV + t * kTileBytes + i * kKPanel, &vmap, kc + 64 * i, y, v_full + 8 * t);
+                ++issued_v;
+            }
+            if (!ok) {
+                // this CTA's copies land before its shared memory is given back
+                mbar_wait(q_full, 0, drain_flag, p.status);
+                for (int j = max(0, issued_k - C::kKS); j < issued_k; ++j)
+                    mbar_wait(k_full + 8 * (j % C::kKS), (j / C::kKS) & 1, drain_flag, p.status);
+                for (int j = max(0, issued_v - C::kVS); j < issued_v; ++j)
+                    mbar_wait(v_full + 8 * (j % C::kVS), (j / C::kVS) & 1, drain_flag, p.status);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        // ================= MMA issuer (the whole warp walks, lane 0 issues) =================
+        constexpr uint32_t kFmt = kF16 ? 0u : 1u;
+        constexpr uint32_t kIdescQK = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kK >> 3) << 17) | ((kQ >> 4) << 24);
+        constexpr uint32_t kIdescPV = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) |
+                                      ((kQ >> 4) << 24);
+        constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
+        bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag, p.status);
+        auto qk = [&](int j) {
+            const int s = j % C::kKS;
+            if (!mbar_wait(k_full + 8 * s, (j / C::kKS) & 1, abort_flag, p.status)) return false;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    mma_bf16(tmem + 64 * (j & 1), sw128_desc(sQ + (ks / 4) * kQPanel + (ks % 4) * 32),
+                             sw128_desc(sK + s * kTileBytes + (ks / 4) * kKPanel + (ks % 4) * 32), kIdescQK, ks > 0);
+                mma_commit(s_full + 8 * (j & 1));
+                mma_commit(k_empty + 8 * s);
+            }
+            return true;
+        };
+        for (int j = 0; j < min(n, 2) && ok; ++j) ok = qk(j);
+        for (int j = 0; j < n && ok; ++j) {
+            const int t = j % C::kVS;
+            const uint32_t v0 = sV + t * kTileBytes;
+            ok = mbar_wait(v_full + 8 * t, (j / C::kVS) & 1, abort_flag, p.status);
+            if (!ok) break;
+            const int rows = rows_of(block_of(j));
+            if (rows < kK) {
+                // V rows that are not the sequence's: zeros (p is 0 there, and 0 * NaN is not)
+                for (int i = 0; i < C::kPanels; ++i)
+                    for (uint32_t a = rows * 128 + lane * 16; a < (uint32_t)kKPanel; a += 32 * 16)
+                        *reinterpret_cast<uint4*>(sm + (v0 - base) + i * kKPanel + a) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            ok = mbar_wait(p_full + 8 * (j & 1), (j >> 1) & 1, abort_flag, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int ks = 0; ks < kK / 16; ++ks)
+                    mma_ts(tmem + C::kOCol, tmem + 64 * (j & 1) + 8 * ks, mn_desc(v0 + ks * 2048), kIdescPV,
+                           (j > 0 || ks > 0) ? 1u : 0u);
+                mma_commit(o_done);
+                mma_commit(v_empty + 8 * t);
+            }
+            if (j + 2 < n) ok = mbar_wait(o_done, j & 1, abort_flag, p.status) && qk(j + 2);
+        }
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, ok)) {
+            // the MMAs issued so far end before their operands are given back
+            if (lane == 0) {
+                mma_commit(drained);
+                mbar_wait(drained, 0, drain_flag, p.status);
+            }
+        }
+    } else {
+        // ================= softmax: thread = query row (TMEM lane) =================
+        const int row = threadIdx.x;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+        const bool live = 32 * warp < q_rows;  // a warp without rows only keeps the barriers' counts
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const uint32_t ts = lane_base + 64 * (j & 1);
+            ok = mbar_wait(s_full + 8 * (j & 1), (j >> 1) & 1, abort_flag, p.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (live) {
+                uint32_t s[2][32];
+                tmem_ld32(ts, s[0]);
+                tmem_ld32(ts + 32, s[1]);
+                tmem_wait_ld();
+                tmem_settle(s[0]);
+                tmem_settle(s[1]);
+                const int rows = rows_of(block_of(j));
+                if (rows < kK) {
+#pragma unroll
+                    for (int i = 0; i < kK; ++i)
+                        if (i >= rows) s[i / 32][i % 32] = 0xff800000u;  // -inf
+                }
+                float mx = m;
+#pragma unroll
+                for (int i = 0; i < kK; i += 2)
+                    mx = max3(mx, __uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
+                // a NaN maximum always counts as grown, and stays
+                const bool grown = !((mx - m) * p.c <= kSlack) && !(mx == -INFINITY);
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float to = grown ? mx : m;
+                    const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
+                    if (j > 0) {
+                        ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, p.status);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(lane_base + C::kOCol + c0, o);
+                            tmem_wait_ld();
+                            tmem_settle(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(lane_base + C::kOCol + c0, o);
+                        }
+                    }
+                    l *= alpha;
+                    m = to;
+                }
+                const float bias = m == -INFINITY ? 0.f : -m * p.c;
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float p0 = exp2_hw(fmaf(__uint_as_float(s[half][2 * i]), p.c, bias));
+                        const float p1 = exp2_hw(fmaf(__uint_as_float(s[half][2 * i + 1]), p.c, bias));
+                        sum0 += p0;
+                        sum1 += p1;
+                        w[i] = pack2<kF16>(p0, p1);
+                    }
+                    tmem_st16(ts + 16 * half, w);
+                }
+                l += sum0 + sum1;
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(p_full + 8 * (j & 1));
+        }
+        if (ok && n > 0) {
+            // o_done's phases one by one: a parity says nothing about a phase two back
+            // (s_full(n - 1) was seen, so phase n - 3 is over)
+            ok = (n < 2 || mbar_wait(o_done, n & 1, abort_flag, p.status)) &&
+                 mbar_wait(o_done, (n - 1) & 1, abort_flag, p.status);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+        }
+        if (ok && live) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(q_row0 + row) * p.out_stride + (int64_t)h * D;
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld32(lane_base + C::kOCol + c0, o);
+                    tmem_wait_ld();
+                    tmem_settle(o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                }
+                if (row < q_rows) {
+                    uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            w[x] = l == 0.f ? 0u
+                                            : pack2<kF16>(__uint_as_float(o[8 * i + 2 * x]) * inv,
+                                                          __uint_as_float(o[8 * i + 2 * x + 1]) * inv);
+                        d4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::kTmemCols));
+    }
+}
+
+// [rows][cols] 16-bit rows, tiles of box_rows x 64 columns with the 128-byte swizzle
+s3d_status encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows,
+                       bool f16, char* error, uint64_t error_capacity) {
+    auto encode = get_encode_fn();
+    if (!encode) return fail(error, error_capacity, S3D_INTERNAL_ERROR, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult cr = encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                               const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS)
+        return fail(error, error_capacity, S3D_INTERNAL_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    return S3D_OK;
+}
+
+template <int D, bool kF16>
+cudaError_t launch(s3dsp_context* ctx, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                   const AttnParams& p) {
+    static std::atomic<uint64_t> optin{0};
+    const cudaError_t e = smem_optin((const void*)block_attention_kernel<D, kF16>, ctx->device, optin);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
+                      ctx->stream, q, k, v, p);
+}
+
+}  // namespace
+
+extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const s3dsp_attn_plan* plan, const void* q,
+                                                      int64_t q_stride, int32_t heads, const void* k, int64_t k_stride,
+                                                      const void* v, int64_t v_stride, int32_t kv_heads,
+                                                      uint32_t dtype, int32_t d, float scale, const int32_t* d_sel,
+                                                      int32_t top, void* out, int64_t out_stride, char* error,
+                                                      uint64_t error_capacity) {
+    clear_error(error, error_capacity);
+    if (!ctx || !plan) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "NULL argument");
+    if (plan->device != ctx->device)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "the plan is on device %d, the context on %d",
+                    plan->device, ctx->device);
+    if (dtype != S3DSP_BF16 && dtype != S3DSP_F16)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "dtype %u (bf16 or f16 supported)", dtype);
+    if (d != 64 && d != 128)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "head dimension %d (64 or 128 supported)", d);
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 4096)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "%d heads over %d key heads", heads, kv_heads);
+    const int64_t qw = (int64_t)heads * d, kw = (int64_t)kv_heads * d;
+    if (q_stride < qw || out_stride < qw || k_stride < kw || v_stride < kw)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "row stride below heads * d");
+    // the tensor maps' row stride: a multiple of 16 bytes below 2^40
+    constexpr int64_t kMaxStride = 1ll << 38;
+    if ((q_stride | k_stride | v_stride | out_stride) & 7 || q_stride > kMaxStride || k_stride > kMaxStride ||
+        v_stride > kMaxStride)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "row strides must be multiples of 8 elements");
+    if (!(scale > 0.f) || std::isinf(scale))
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "scale must be positive and finite");
+    if (d_sel ? (top < 1 || top > kAttnMaxTop) : top != 0)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "top %d (1 to %d with a selection, else 0)", top,
+                    kAttnMaxTop);
+    if (plan->n_qb == 0) return S3D_OK;
+    if (!q || !out || (plan->n_k > 0 && (!k || !v)))
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "NULL argument");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointers need 16-byte alignment");
+    S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
+    const bool f16 = dtype == S3DSP_F16;
+    CUtensorMap qm, km, vm;
+    S3DSP_TRY(encode_rows(&qm, q, plan->n_q, qw, q_stride, kQ, f16, error, error_capacity));
+    // a plan without key rows lists nothing: its maps are never read through
+    const bool keys = plan->n_k > 0;
+    S3DSP_TRY(encode_rows(&km, keys ? k : q, keys ? plan->n_k : 1, kw, k_stride, kK, f16, error, error_capacity));
+    S3DSP_TRY(encode_rows(&vm, keys ? v : q, keys ? plan->n_k : 1, kw, v_stride, kK, f16, error, error_capacity));
+    AttnParams p = {plan->q_blocks, d_sel, top, heads, heads / kv_heads, scale * 1.4426950408889634f,
+                    out, out_stride, ctx->d_status};
+    const dim3 grid((unsigned)plan->n_qb, (unsigned)heads);
+    const cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p) : launch<64, false>(ctx, grid, qm, km, vm, p))
+                                  : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p)
+                                         : launch<128, false>(ctx, grid, qm, km, vm, p));
+    if (e != cudaSuccess) return cuda_fail(error, error_capacity, e, "block_attention_kernel");
+    return S3D_OK;
+}

@@ -78,7 +78,32 @@ struct s3dsp_kmap {
     int64_t n_tiles = 0;
 };
 
+// A ragged attention batch cut into blocks (s3dsp_attn_plan_create): one device
+// allocation holding the tables below.
+struct s3dsp_attn_plan {
+    int device = 0;
+    bool self = false;               // the key rows are the query rows
+    int64_t n_q = 0, n_k = 0;        // rows the plan spans (the last offsets)
+    int64_t n_seq = 0;
+    int n_qb = 0, n_kb = 0, n_groups = 0, n_pairs = 0;
+    int max_kb = 0;                  // most key blocks of a sequence
+    int group = 1;                   // query blocks of a selection group
+    void* mem = nullptr;
+    int4* q_blocks = nullptr;        // [n_qb] {first row, rows | index in the sequence << 8, first key row, key rows}
+    int2* k_blocks = nullptr;        // [n_kb] {first row, rows}
+    int2* groups = nullptr;          // [n_groups] {first query block, up to `group` blocks of one sequence}
+    int2* pairs = nullptr;           // [n_pairs] {first query block, 1 or 2 blocks of one sequence}
+    int* first_kb = nullptr;         // [n_qb] first key block of the block's sequence
+};
+
 namespace s3dsp {
+
+constexpr int kAttnQRows = 128;      // rows of a query block (tcgen05 M)
+constexpr int kAttnKRows = 64;       // rows of a key block
+constexpr int kAttnRowsBits = 8;     // s3dsp_attn_plan::q_blocks[].y: rows below, index above
+constexpr int kAttnRowsMask = (1 << kAttnRowsBits) - 1;
+constexpr int kAttnGroupRows = 16;   // most query blocks whose block scores are computed together
+constexpr int kAttnMaxTop = 1024;    // longest list of key blocks
 
 constexpr int kTileRows = 128;  // rows per conv tile (tcgen05 M) == tile_mask granularity
 constexpr int kSmemOptIn = 232448;  // opt-in dynamic shared memory per block (227 KB)

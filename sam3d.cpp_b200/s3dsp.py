@@ -27,6 +27,8 @@ SENTINEL_SLAT_N, SENTINEL_MESH_NEG1 = 0, 1
 EPI_SILU, PRO_AFFINE_SILU, CONV_CTA_PAIR, CONV_TILE128, CONV_STREAM_K, CONV_STREAM_K128, EPI_GELU = 1, 2, 4, 8, 16, 32, 64
 CONV_SPLIT_PAIRS = 128
 CONV_HALO = 256
+ROPE_HALF, ROPE_INVERSE, QK_GAMMA_SHARED = 1, 2, 4
+ATTN_Q_ROWS, ATTN_K_ROWS = 128, 64
 CONTEXT_DEFERRED_CHECKS = 1
 CONTEXT_OWN_STREAM = 2
 CONTEXT_COPY_STREAMS = 4
@@ -37,6 +39,8 @@ EXPORTED = [
     "s3dsp_context_check", "s3dsp_context_fork", "s3dsp_context_join", "s3dsp_memory_stats", "s3dsp_device_alloc", "s3dsp_device_free", "s3dsp_copy_to_device",
     "s3dsp_copy_to_host", "s3dsp_hash_build", "s3dsp_hash_free", "s3dsp_hash_size",
     "s3dsp_hash_lookup", "s3dsp_gs_window_tables", "s3dsp_ape", "s3dsp_gather_rows", "s3dsp_window_attention", "s3dsp_flexicubes_tables_create",
+    "s3dsp_rope", "s3dsp_qk_norm_rope", "s3dsp_attn_plan_create", "s3dsp_attn_plan_free", "s3dsp_attn_plan_info",
+    "s3dsp_block_select", "s3dsp_block_attention",
     "s3dsp_flexicubes_tables_free", "s3dsp_flexicubes_extract", "s3dsp_mesh_info", "s3dsp_mesh_device", "s3dsp_mesh_copy",
     "s3dsp_mesh_free", "s3dsp_gguf_open", "s3dsp_gguf_close", "s3dsp_gguf_n_tensors", "s3dsp_gguf_find",
     "s3dsp_gguf_tensor_info", "s3dsp_gguf_u32", "s3dsp_gguf_i32", "s3dsp_gguf_f32", "s3dsp_gguf_str",
@@ -71,6 +75,7 @@ _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _cp = ctypes.c_char_p
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 
 def load(path: str = LIB_PATH):
@@ -105,6 +110,17 @@ def load(path: str = LIB_PATH):
         "s3dsp_ape": (_u32, [_vp, _vp, _i64, _i32, _vp, _cp, _u64]),
         "s3dsp_gather_rows": (_u32, [_vp, _vp, _u32, _i64, _i64, _vp, _i64, _vp, _u32, _cp, _u64]),
         "s3dsp_window_attention": (_u32, [_vp, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _cp, _u64]),
+        "s3dsp_rope": (_u32, [_vp, _vp, _u32, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _d, _u32, _vp, _u32, _i64,
+                              _cp, _u64]),
+        "s3dsp_qk_norm_rope": (_u32, [_vp, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _u32, _i64, _i32, _f, _vp, _i64,
+                                      _i32, _vp, _d, _u32, _vp, _i64, _vp, _i64, _u32, _cp, _u64]),
+        "s3dsp_attn_plan_create": (_u32, [_vp, _vp, _vp, _i64, ctypes.POINTER(_vp), _cp, _u64]),
+        "s3dsp_attn_plan_free": (None, [_vp, _vp]),
+        "s3dsp_attn_plan_info": (_u32, [_vp] + [ctypes.POINTER(_i64)] * 5),
+        "s3dsp_block_select": (_u32, [_vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _u32, _i32, _i32, _i32, _vp, _cp,
+                                      _u64]),
+        "s3dsp_block_attention": (_u32, [_vp, _vp, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _u32, _i32, _f, _vp,
+                                         _i32, _vp, _i64, _cp, _u64]),
         "s3dsp_flexicubes_tables_create": (_u32, [_vp, _vp, _vp, _vp, ctypes.POINTER(_vp), _cp, _u64]),
         "s3dsp_flexicubes_tables_free": (None, [_vp, _vp]),
         "s3dsp_flexicubes_extract": (_u32, [_vp, _vp, _vp, _vp, _i64, ctypes.POINTER(_vp), _cp, _u64]),
@@ -219,6 +235,24 @@ def dtype_code(t) -> int:
     return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}[t.dtype]
 
 
+def _rows(t, name: str):
+    """(address, row stride) of a 2-D tensor whose columns are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: rows of contiguous columns are wanted")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
+
+
+def _head_dim(t, heads: int, name: str) -> int:
+    if heads <= 0 or t.shape[1] % heads:
+        raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: {t.shape[1]} columns are no {heads} heads")
+    return t.shape[1] // heads
+
+
+def _same(what: str, *vals):
+    if any(v != vals[0] for v in vals[1:]):
+        raise S3dError(S3D_INVALID_ARGUMENT, f"{what} differ: {vals}")
+
+
 class Kmap:
     def __init__(self, ctx: "Context", handle: int, rows: int):
         self.ctx, self.handle, self.rows = ctx, handle, rows
@@ -262,6 +296,27 @@ class SlatTables:
     def free(self):
         if self.handle:
             load().s3dsp_slat_tables_free(self.ctx.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class AttnPlan:
+    """Block tables of a ragged attention batch (s3dsp_attn_plan_create)."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self.handle = ctx, handle
+        c = [_i64() for _ in range(5)]
+        load().s3dsp_attn_plan_info(handle, *(ctypes.byref(v) for v in c))
+        self.n_q, self.n_k, self.q_blocks, self.k_blocks, self.max_k_blocks = (v.value for v in c)
+
+    def free(self):
+        if self.handle:
+            load().s3dsp_attn_plan_free(self.ctx.handle, self.handle)
             self.handle = None
 
     def __del__(self):
@@ -605,6 +660,113 @@ class Context:
         device int32 [nw, 2] (first row, rows); row i to out[scatter[i]]."""
         _call(load().s3dsp_window_attention, self.handle, ptr(qkv), qkv.shape[0], qkv.shape[1] // 3, heads,
               ptr(windows), windows.shape[0], ptr(scatter), ptr(out))
+
+    # ---- attention over voxel tokens ----------------------------------------
+    @staticmethod
+    def _positions(positions, axis_pairs, n):
+        """(address, row stride, axes, host axis_pairs) of int32 positions [n, >= axes]."""
+        import torch
+        axes = len(axis_pairs)
+        if axes == 0:
+            return None, 0, 0, None
+        if positions is None or positions.dim() != 2 or positions.dtype != torch.int32 or positions.shape[0] != n \
+                or positions.shape[1] < axes or (positions.shape[1] > 1 and positions.stride(1) != 1):
+            raise S3dError(S3D_INVALID_ARGUMENT, f"positions: int32 [{n}, >= {axes}] rows are wanted")
+        stride = positions.stride(0) if n > 1 else max(positions.stride(0), positions.shape[1])
+        return positions.data_ptr(), stride, axes, (_i32 * axes)(*axis_pairs)
+
+    def rope(self, x, positions, heads: int, out, axis_pairs, theta: float = 10000.0, half: bool = False,
+             inverse: bool = False):
+        """out = x [n, heads * d] with every head turned by positions (int32
+        [n, axes]); axis_pairs: pairs of each axis. Rows may be strided."""
+        d = _head_dim(x, heads, "x")
+        _same("x and out", tuple(x.shape), tuple(out.shape))
+        xp, xs = _rows(x, "x")
+        yp, ys = _rows(out, "out")
+        pos, pst, axes, pairs = self._positions(positions, axis_pairs, x.shape[0])
+        _call(load().s3dsp_rope, self.handle, xp, dtype_code(x), x.shape[0], xs, heads, d, pos, pst, axes, pairs, theta,
+              (ROPE_HALF if half else 0) | (ROPE_INVERSE if inverse else 0), yp, dtype_code(out), ys)
+
+    def qk_norm_rope(self, q, heads: int, q_gamma, q_out, k=None, kv_heads: int = 0, k_gamma=None, k_out=None,
+                     eps: float = 1e-6, positions=None, axis_pairs=(), theta: float = 10000.0, half: bool = False):
+        """RMS norm of every head of q (and k) with weights f32 [heads, d] (or
+        [d] for all heads, or None), then the rotation (axis_pairs () : none)."""
+        import torch
+        n, d = q.shape[0], _head_dim(q, heads, "q")
+        _same("q and q_out", tuple(q.shape), tuple(q_out.shape))
+        qp, qs = _rows(q, "q")
+        qop, qos = _rows(q_out, "q_out")
+        kp = kop = None
+        ks = kos = 0
+        flags = ROPE_HALF if half else 0
+        if k is not None:
+            _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
+            _same("rows and types", (n, q.dtype), (k.shape[0], k.dtype))
+            _same("k and k_out", tuple(k.shape), tuple(k_out.shape))
+            _same("output types", q_out.dtype, k_out.dtype)
+            kp, ks = _rows(k, "k")
+            kop, kos = _rows(k_out, "k_out")
+        gammas = [(g, h) for g, h in ((q_gamma, heads), (k_gamma, kv_heads)) if g is not None]
+        if any(g.dim() == 1 for g, _ in gammas):
+            flags |= QK_GAMMA_SHARED
+        for g, h in gammas:
+            want = (d,) if flags & QK_GAMMA_SHARED else (h, d)
+            if tuple(g.shape) != want or g.dtype != torch.float32 or not g.is_contiguous():
+                raise S3dError(S3D_INVALID_ARGUMENT, f"gamma: contiguous float32 {want} is wanted")
+        pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
+        _call(load().s3dsp_qk_norm_rope, self.handle, qp, qs, heads, ptr(q_gamma), kp, ks, kv_heads, ptr(k_gamma),
+              dtype_code(q), n, d, eps, pos, pst, axes, pairs, theta, flags, qop, qos, kop, kos, dtype_code(q_out))
+
+    def attn_plan(self, q_offsets, k_offsets=None) -> AttnPlan:
+        """Plan of a ragged batch: host offsets [n_seq + 1] of the sequences'
+        query rows, and of their key rows (None: the same rows)."""
+        import numpy as np
+        qo = np.ascontiguousarray(q_offsets, dtype=np.int64).reshape(-1)
+        ko = None if k_offsets is None else np.ascontiguousarray(k_offsets, dtype=np.int64).reshape(-1)
+        if len(qo) < 1 or (ko is not None and len(ko) != len(qo)):
+            raise S3dError(S3D_INVALID_ARGUMENT, "offsets: n_seq + 1 values each")
+        h = _vp()
+        _call(load().s3dsp_attn_plan_create, self.handle, qo.ctypes.data, ko.ctypes.data if ko is not None else None,
+              len(qo) - 1, ctypes.byref(h))
+        return AttnPlan(self, h.value)
+
+    @staticmethod
+    def _attn_rows(plan: AttnPlan, q, heads: int, k, kv_heads: int):
+        d = _head_dim(q, heads, "q")
+        _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
+        _same("types of q and k", q.dtype, k.dtype)
+        if q.shape[0] < plan.n_q or k.shape[0] < plan.n_k:
+            raise S3dError(S3D_INVALID_ARGUMENT, f"the plan spans {plan.n_q} query rows and {plan.n_k} key rows")
+        return d
+
+    def block_select(self, plan: AttnPlan, q, k, heads: int, kv_heads: int, sel, keep_local: bool = False):
+        """sel (device int32 [plan.q_blocks, heads, top]) = the key blocks with the largest scores."""
+        import torch
+        d = self._attn_rows(plan, q, heads, k, kv_heads)
+        if sel.dim() != 3 or sel.dtype != torch.int32 or not sel.is_contiguous() or \
+                tuple(sel.shape[:2]) != (plan.q_blocks, heads):
+            raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
+        qp, qs = _rows(q, "q")
+        kp, ks = _rows(k, "k")
+        _call(load().s3dsp_block_select, self.handle, plan.handle, qp, qs, heads, kp, ks, kv_heads, dtype_code(q), d,
+              sel.shape[2], int(keep_local), ptr(sel))
+
+    def block_attention(self, plan: AttnPlan, q, k, v, heads: int, kv_heads: int, out, scale: float | None = None,
+                        sel=None):
+        """out = softmax(scale q k^T over the listed key blocks (sel None: all)) v; scale None: 1 / sqrt(d)."""
+        import torch
+        d = self._attn_rows(plan, q, heads, k, kv_heads)
+        _same("k and v", (tuple(k.shape), k.dtype), (tuple(v.shape), v.dtype))
+        _same("q and out", (tuple(q.shape), q.dtype), (tuple(out.shape), out.dtype))
+        top = 0
+        if sel is not None:
+            if sel.dim() != 3 or sel.dtype != torch.int32 or not sel.is_contiguous() or \
+                    tuple(sel.shape[:2]) != (plan.q_blocks, heads):
+                raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
+            top = sel.shape[2]
+        (qp, qs), (kp, ks), (vp, vs), (op, os_) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
+        _call(load().s3dsp_block_attention, self.handle, plan.handle, qp, qs, heads, kp, ks, vp, vs, kv_heads,
+              dtype_code(q), d, d ** -0.5 if scale is None else scale, ptr(sel), top, op, os_)
 
     # ---- FlexiCubes extraction ---------------------------------------------
     def flexicubes_tables(self, dmc, num_dual, check) -> FlexiCubesTables:

@@ -1,0 +1,705 @@
+"""The attention operators over voxel tokens against their definitions in 64
+bits: s3dsp_rope, s3dsp_qk_norm_rope, s3dsp_block_select, s3dsp_block_attention
+alone, at the sizes and masks where they can go wrong, and run together.
+
+Tolerances count roundings (u = eps / 2 of the output type, 2^-24 an f32 one):
+
+rope      an angle's remainder is rounded once (at most half a turn: pi 2^-25), sincospif is within 2 ulp
+          (2^-23), two products and a sum follow: below (|a| + |b|) 6 * 2^-24 before the output's rounding.
+          The f64 angle itself: frequency / 2 pi carries a pow (1 ulp: 2^-52), the constant 2 pi and a division
+          (2^-53 each), the product with the position 2^-53; the definition here a pow and a product (2^-53 each):
+          together at most |pos| 7 * 2^-53 of the pair's size (1.7e-6 at 2^31, nothing at voxel positions).
+qk        the mean square adds at most 8 + 5 additions, a division, a sum, a square root, a division and
+          two products: below 20 roundings more on each value.
+attention P is rounded to the type (u of sum p |v| / sum p); a score errs by the f32 accumulation of d products,
+          which may truncate (d 2^-23 sum |q k| scale), its exponential by that and a few 2^-22, in the
+          numerator and in the sum; then the output's rounding.
+"""
+import numpy as np
+import pytest
+import torch
+
+import s3dsp
+import workloads
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+F32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return s3dsp.Context(0)
+
+
+def randn(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def strided(shape, seed, dtype, pad=0, offset=0, scale=1.0):
+    """Rows inside a wider buffer, `offset` elements in."""
+    n, w = shape
+    return randn((n, w + pad + offset), seed, dtype, scale)[:, offset:offset + w]
+
+
+def within(got, want, tol, u):
+    """|got - want| <= tol + u |want|, elementwise (f16 adds its smallest step)."""
+    got = got.double()
+    tiny = 2.0 ** -24 if u == 2.0 ** -11 else 2.0 ** -133
+    off = (got - want).abs() - (tol + u * (want.abs() + tol) + tiny)
+    assert torch.isfinite(got).all()
+    worst = int(off.argmax())
+    assert off.max() <= 0, f"off by {float((got - want).abs().flatten()[worst]):.3e} at {worst}, want {float(want.flatten()[worst]):.6e}"
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ---------------------------------------------------------------------------------------------------
+# rope, qk_norm_rope
+# ---------------------------------------------------------------------------------------------------
+def turned(x, pos, heads, pairs, theta, half, inverse):
+    """x [n, heads * d] f64 turned, and |a| + |b| of each value's pair."""
+    n, d = x.shape[0], x.shape[1] // heads
+    x = x.reshape(n, heads, d)
+    y, size = x.clone(), x.abs()
+    j = 0
+    for a, p in enumerate(pairs):
+        for i in range(p):
+            ang = pos[:, a].double() * theta ** (-i / p)
+            c, s = ang.cos()[:, None], ang.sin()[:, None] * (-1 if inverse else 1)
+            i0, i1 = (j, j + d // 2) if half else (2 * j, 2 * j + 1)
+            y[:, :, i0], y[:, :, i1] = x[:, :, i0] * c - x[:, :, i1] * s, x[:, :, i0] * s + x[:, :, i1] * c
+            size[:, :, i0] = size[:, :, i1] = x[:, :, i0].abs() + x[:, :, i1].abs()
+            j += 1
+    return y.reshape(n, heads * d), size.reshape(n, heads * d)
+
+
+ROPE = [
+    # n, heads, d, pairs, in, out, pad, offset, span
+    (1, 1, 8, [1, 1, 1], "f32", "f32", 0, 0, 64),
+    (5, 3, 64, [10, 10, 10], "bf16", "bf16", 0, 0, 64),
+    (1000, 12, 64, [10, 10, 10], "bf16", "bf16", 0, 0, 32768),
+    (777, 16, 128, [21, 21, 21], "f16", "f16", 8, 0, 64),
+    (300, 4, 96, [48], "f32", "bf16", 0, 0, 2 ** 31 - 1),
+    (300, 4, 80, [0, 40], "bf16", "f32", 3, 1, 2 ** 31 - 1),
+    (131, 2, 256, [32, 32, 32, 32], "f32", "f32", 1, 3, 1000),
+    (64, 5, 24, [2, 3, 4], "f16", "bf16", 5, 0, 100),
+    (9, 70, 64, [16, 16], "bf16", "f16", 0, 8, 100),
+    (40, 2, 64, [], "bf16", "bf16", 0, 0, 100),
+]
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("n,heads,d,pairs,di,do,pad,offset,span", ROPE)
+def test_rope(ctx, n, heads, d, pairs, di, do, pad, offset, span, half, inverse):
+    x = strided((n, heads * d), 1, DT[di], pad, offset, 1.7)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    pos = torch.randint(-span, span, (n, 5), generator=g, device="cuda", dtype=torch.int32)[:, 1:]
+    keep = torch.full((n, heads * d + pad), 7.0, dtype=DT[do], device="cuda")
+    out = keep[:, :heads * d]
+    ctx.rope(x, pos, heads, out, pairs, theta=100.0, half=half, inverse=inverse)
+    want, size = turned(x.double(), pos, heads, pairs, 100.0, half, inverse)
+    within(out, want, size * (6 * F32 + span * 7 * 2.0 ** -53), unit(DT[do]))
+    assert (keep[:, heads * d:] == 7.0).all()
+
+
+def test_rope_in_place_and_back(ctx):
+    """In place, then by the inverse: the rows come back; and the inverse is the transpose (what a gradient takes)."""
+    n, heads, d, pairs = 500, 4, 64, [10, 10, 10]
+    x = randn((n, heads * d), 3)
+    pos = torch.randint(0, 64, (n, 3), device="cuda", dtype=torch.int32)
+    y = x.clone()
+    ctx.rope(y, pos, heads, y, pairs)
+    back = torch.empty_like(y)
+    ctx.rope(y, pos, heads, back, pairs, inverse=True)
+    size = turned(x.double(), pos, heads, pairs, 1e4, False, False)[1]
+    assert ((back - x).double().abs() <= 4 * 6 * F32 * size).all()
+    w = randn((n, heads * d), 4)
+    wt = torch.empty_like(w)
+    ctx.rope(w, pos, heads, wt, pairs, inverse=True)
+    a, b = (w.double() * y.double()).sum(), (wt.double() * x.double()).sum()  # <w, R x> = <R^T w, x>
+    assert abs(a - b) <= 2 * 6 * F32 * float((w.abs() * 2 * size).sum())
+    # and against differences along a direction: R is linear
+    e = randn((n, heads * d), 5)
+    y2 = torch.empty_like(y)
+    ctx.rope(x + e, pos, heads, y2, pairs)
+    diff = (w.double() * (y2.double() - y.double())).sum()
+    assert abs(diff - (wt.double() * ((x + e).double() - x.double())).sum()) <= 6 * 6 * F32 * float((w.abs() * 3 * size).sum()) + \
+        6 * 6 * F32 * float((w.abs() * e.abs()).sum() * 3)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("gamma", ["heads", "shared", "none"])
+@pytest.mark.parametrize("n,heads,kv,d,pairs,di,do,pad,offset", [
+    (1, 2, 1, 64, [10, 10, 10], "bf16", "bf16", 0, 0),
+    (2500, 12, 12, 64, [10, 10, 10], "bf16", "bf16", 1536, 0),
+    (311, 16, 4, 128, [21, 21, 21], "f32", "bf16", 0, 0),
+    (100, 3, 0, 40, [20], "f16", "f32", 1, 1),
+    (77, 6, 2, 256, [], "bf16", "f16", 0, 0),
+])
+def test_qk_norm_rope(ctx, n, heads, kv, d, pairs, di, do, pad, offset, gamma, half):
+    q = strided((n, heads * d), 1, DT[di], pad, offset, 2.0)
+    k = strided((n, kv * d), 2, DT[di], pad, offset, 0.01) if kv else None
+    pos = torch.randint(0, 64, (n, 4), device="cuda", dtype=torch.int32)
+    shape = {"heads": lambda h: (h, d), "shared": lambda h: (d,)}.get(gamma)
+    gq = randn(shape(heads), 5, scale=0.3) + 1.0 if shape else None
+    gk = randn(shape(kv), 6, scale=0.3) + 1.0 if shape and kv else None
+    qo = torch.empty((n, heads * d), dtype=DT[do], device="cuda")
+    ko = torch.empty((n, kv * d), dtype=DT[do], device="cuda") if kv else None
+    ctx.qk_norm_rope(q, heads, gq, qo, k, kv, gk, ko, eps=1e-6, positions=pos[:, 1:], axis_pairs=pairs, half=half)
+    for x, g, h, out in [(q, gq, heads, qo)] + ([(k, gk, kv, ko)] if kv else []):
+        x = x.double().reshape(n, h, d)
+        x = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+        x = (x if g is None else x * g.double()).reshape(n, h * d)
+        want, size = turned(x, pos[:, 1:], h, pairs, 1e4, half, False)
+        within(out, want, size * (6 + 20) * F32, unit(DT[do]))
+
+
+def test_qk_norm_of_zero_rows_and_in_place(ctx):
+    x = torch.zeros((3, 128), dtype=torch.bfloat16, device="cuda")
+    ctx.qk_norm_rope(x, 2, None, x)
+    assert (x == 0).all()  # 0 / sqrt(eps)
+    ctx.qk_norm_rope(x[:0], 2, None, x[:0])
+
+
+def test_rows_beyond_32_bits(ctx):
+    """Rows whose element offsets pass 2^32: each is where its stride says."""
+    n, stride = 40000, 120000
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    big = torch.empty((n, stride), dtype=torch.bfloat16, device="cuda")
+    x = big[:, 64:192]
+    x.copy_(randn((n, 128), 1, torch.bfloat16))
+    src = x.clone()
+    pos = torch.randint(0, 64, (n, 3), device="cuda", dtype=torch.int32)
+    out, ref = torch.empty_like(src), torch.empty_like(src)
+    ctx.rope(x, pos, 2, out, [10, 10, 10])
+    ctx.rope(src, pos, 2, ref, [10, 10, 10])
+    assert torch.equal(out, ref)
+    plan = ctx.attn_plan([0, 30000, n])
+    sel, sref = (torch.empty((plan.q_blocks, 2, 4), dtype=torch.int32, device="cuda") for _ in range(2))
+    ctx.block_select(plan, x, x, 2, 2, sel)
+    ctx.block_select(plan, src, src, 2, 2, sref)
+    assert torch.equal(sel, sref)
+    ctx.block_attention(plan, x, x, x, 2, 2, out, sel=sel)
+    ctx.block_attention(plan, src, src, src, 2, 2, ref, sel=sel)
+    assert torch.equal(out, ref)
+    wide = big[:, 256:384]
+    ctx.block_attention(plan, src, src, src, 2, 2, wide, sel=sel)
+    assert torch.equal(wide, ref)
+    ctx.check()
+
+
+# ---------------------------------------------------------------------------------------------------
+# block_select
+# ---------------------------------------------------------------------------------------------------
+def offsets(lens, start=0):
+    return np.concatenate([[0], np.cumsum(lens)]) + start
+
+
+def chosen(q, k, lens, klens, heads, kv, top, local):
+    """The selection by its definition: f64 means and scores, numpy's stable sort."""
+    q, k = q.double(), k.double()
+    d = q.shape[1] // heads
+    rows, q0, k0 = [], 0, 0
+    for m, mk in zip(lens, klens):
+        nb, nk = -(-m // 128), -(-mk // 64)
+        qm = torch.stack([q[q0 + 128 * b:q0 + min(m, 128 * b + 128)].mean(0) for b in range(nb)]) if nb else q[:0]
+        km = torch.stack([k[k0 + 64 * c:k0 + min(mk, 64 * c + 64)].mean(0) for c in range(nk)]) if nk else k[:0]
+        qm = qm.reshape(nb, heads, d).permute(1, 0, 2)
+        km = km.reshape(nk, kv, d).permute(1, 0, 2).repeat_interleave(heads // kv, 0)
+        score = torch.where((s := qm @ km.transpose(1, 2)).isnan(), -torch.inf, s).cpu().numpy()
+        for b in range(nb):
+            if local:
+                score[:, b, 2 * b:2 * b + 2] = np.inf
+            order = np.argsort(-score[:, b], axis=1, kind="stable")[:, :top]
+            pad = np.full((heads, top - order.shape[1]), -1)
+            rows.append(np.concatenate([np.sort(order, axis=1), pad], axis=1))
+        q0, k0 = q0 + m, k0 + mk
+    return torch.from_numpy(np.array(rows, np.int32).reshape(-1, heads, top))
+
+
+SELECT = [
+    # lens, klens, heads, kv, d, dtype, top, local, pad, offset
+    ([1], None, 1, 1, 64, "bf16", 1, False, 0, 0),
+    ([1000], None, 4, 4, 64, "bf16", 5, True, 0, 0),
+    ([1000], None, 4, 2, 128, "f32", 5, False, 3, 1),
+    ([0, 700, 1, 0, 129, 64, 5000], None, 6, 3, 64, "f16", 9, True, 8, 0),
+    ([300, 20], [5000, 64], 2, 1, 64, "bf16", 16, False, 0, 0),
+    ([300, 20, 5], [0, 640, 65], 2, 2, 40, "bf16", 3, False, 1, 0),
+    ([2600], None, 3, 3, 256, "bf16", 1024, False, 0, 0),
+    ([9000], None, 2, 2, 64, "bf16", 64, True, 0, 0),
+]
+
+
+@pytest.mark.parametrize("lens,klens,heads,kv,d,dt,top,local,pad,offset", SELECT)
+def test_block_select(ctx, lens, klens, heads, kv, d, dt, top, local, pad, offset):
+    q = strided((sum(lens), heads * d), 1, DT[dt], pad, offset)
+    k = strided((sum(klens or lens), kv * d), 2, DT[dt], pad, offset)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens) if klens else None)
+    sel = torch.full((plan.q_blocks, heads, top), -7, dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, heads, kv, sel, keep_local=local)
+    assert torch.equal(sel.cpu(), chosen(q, k, lens, klens or lens, heads, kv, top, local))
+
+
+def test_block_select_ties_and_nan(ctx):
+    """Equal scores (whole numbers, exact in any order, and signed zeros): the lowest index; NaN scores last."""
+    n, top = 64 * 40, 7
+    q = torch.ones((n, 64), device="cuda")
+    k = torch.zeros((n, 64), device="cuda")
+    level = torch.tensor([3, 1, 2, 2, 0, 3, 2, 2, 2, 1] * 4, dtype=torch.float32)
+    k[:, 0] = level.repeat_interleave(64).cuda()
+    plan = ctx.attn_plan([0, n])
+    sel = torch.empty((plan.q_blocks, 1, top), dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, 1, 1, sel)
+    want = np.sort(np.argsort(-level.numpy(), kind="stable")[:top])
+    assert (sel.cpu().numpy() == want).all(), sel[0]
+    k.zero_()
+    k[64 * 3:64 * 5] = -0.0
+    ctx.block_select(plan, q, k, 1, 1, sel)
+    assert (sel.cpu().numpy() == np.arange(top)).all()
+    k[:64 * 38] = float("nan")
+    ctx.block_select(plan, q, k, 1, 1, sel)
+    assert (sel.cpu().numpy() == np.array([0, 1, 2, 3, 4, 38, 39])).all()
+    k.fill_(-float("inf"))
+    ctx.block_select(plan, q, k, 1, 1, sel)
+    assert (sel.cpu().numpy() == np.arange(top)).all()
+
+
+@pytest.mark.parametrize("n", [120000, 300000])
+def test_block_select_long_sequence(ctx, n):
+    """More key blocks than sixteen score rows leave room for (groups of fewer query blocks)."""
+    q, k = randn((200, 64), 1, torch.bfloat16), randn((n, 64), 2, torch.bfloat16)
+    plan = ctx.attn_plan([0, 200], [0, n])
+    sel = torch.empty((plan.q_blocks, 1, 50), dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, 1, 1, sel)
+    assert torch.equal(sel.cpu(), chosen(q, k, [200], [n], 1, 1, 50, False))
+
+
+def test_block_select_refuses_too_long_a_sequence(ctx):
+    q = torch.zeros((1, 64), device="cuda")
+    k = torch.zeros((1, 64), device="cuda").expand(1 << 21, 64)  # never read
+    plan = ctx.attn_plan([0, 1], [0, 1 << 21])
+    with pytest.raises(s3dsp.S3dError, match="key blocks"):
+        s3dsp._call(s3dsp.load().s3dsp_block_select, ctx.handle, plan.handle, q.data_ptr(), 64, 1, k.data_ptr(), 64, 1,
+                    s3dsp.F32, 64, 4, 0, q.data_ptr())
+
+
+# ---------------------------------------------------------------------------------------------------
+# block_attention
+# ---------------------------------------------------------------------------------------------------
+def attention(q, k, v, lens, klens, heads, kv, scale, sel=None):
+    """The definition in f64, block by block, and the tolerance's two sums: out, sum p |v| / sum p, max sum |q k| scale."""
+    d = q.shape[1] // heads
+    out = torch.zeros((sum(lens), heads, d), dtype=torch.float64, device="cuda")
+    mass, size = torch.zeros_like(out), torch.zeros((sum(lens), heads, 1), dtype=torch.float64, device="cuda")
+    q0 = k0 = b0 = 0
+    for m, mk in zip(lens, klens):
+        nb, nk = -(-m // 128), -(-mk // 64)
+        kh = k[k0:k0 + mk].double().reshape(mk, kv, d).repeat_interleave(heads // kv, 1)
+        vh = v[k0:k0 + mk].double().reshape(mk, kv, d).repeat_interleave(heads // kv, 1)
+        for b in range(nb if mk else 0):
+            r = slice(q0 + 128 * b, q0 + min(m, 128 * b + 128))
+            qh = q[r].double().reshape(-1, heads, d)
+            for h in range(heads):
+                if sel is None:
+                    rows = torch.arange(mk, device="cuda")
+                else:
+                    rows = [torch.arange(64 * c, min(mk, 64 * c + 64), device="cuda") for c in sel[b0 + b, h].tolist() if 0 <= c < nk]
+                    if not rows:
+                        continue
+                    rows = torch.cat(rows)
+                s = qh[:, h] @ kh[rows, h].T * scale
+                p = torch.softmax(s, dim=1)
+                out[r, h], mass[r, h] = p @ vh[rows, h], p @ vh[rows, h].abs()
+                size[r, h, 0] = (qh[:, h].abs() @ kh[rows, h].abs().T).amax(1) * scale
+        q0, k0, b0 = q0 + m, k0 + mk, b0 + nb
+    return out.flatten(1), (mass, size)
+
+
+def check(got, q, k, v, lens, klens, heads, kv, scale, sel=None):
+    want, (mass, size) = attention(q, k, v, lens, klens, heads, kv, scale, sel)
+    d, u = q.shape[1] // heads, unit(q.dtype)
+    tol = (mass * (u + 2 * (size * d * 2.0 ** -23 + 4 * 2.0 ** -22) + 16 * F32)).flatten(1)
+    # f16: weights below the smallest step of f16 (2^-24) are lost or rounded to it
+    if q.dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * v.abs().max().double() * max(klens)
+    within(got, want, tol, u)
+
+
+def lists(plan, heads, top, lens, klens, seed, holes=True):
+    """Random lists without order, with -1 anywhere."""
+    g = np.random.default_rng(seed)
+    sel = np.full((plan.q_blocks, heads, top), -1, np.int32)
+    b = 0
+    for m, mk in zip(lens, klens):
+        nk = -(-mk // 64)
+        for _ in range(-(-m // 128)):
+            for h in range(heads):
+                pick = g.permutation(nk)[:top]
+                at = np.sort(g.permutation(top)[:len(pick)])
+                sel[b, h, at] = pick
+                if holes and top > 1:
+                    sel[b, h, g.random(top) < 0.2] = -1
+            b += 1
+    return torch.from_numpy(sel).cuda()
+
+
+ATTEND = [
+    # lens, klens, heads, kv, d, top, pad
+    ([1], None, 1, 1, 64, 0, 0),
+    ([1], [64], 1, 1, 64, 0, 0),
+    ([5], [63], 2, 1, 64, 0, 8),
+    ([64], [65], 1, 1, 128, 0, 0),
+    ([128], None, 1, 1, 64, 0, 0),
+    ([129], [128], 3, 3, 128, 0, 24),
+    ([1000], None, 12, 12, 64, 0, 1536),
+    ([2000], None, 4, 2, 128, 0, 0),
+    ([0, 300, 1, 0, 77, 640], None, 4, 4, 64, 0, 0),
+    ([0, 300, 1, 0, 77, 640], None, 4, 2, 128, 4, 8),
+    ([1, 1, 1, 1], [700, 1, 64, 5000], 8, 2, 64, 0, 0),
+    ([1, 1, 1], [700, 1, 3000], 8, 2, 128, 8, 0),
+    ([3, 200, 40], [0, 1000, 130], 2, 2, 64, 0, 0),
+    ([3, 200, 40], [0, 1000, 130], 2, 2, 64, 3, 0),
+    ([1500], None, 6, 6, 64, 1, 0),
+    ([1500], None, 6, 3, 64, 40, 0),
+    ([1500], None, 2, 2, 128, 1024, 0),
+    ([4000], None, 2, 2, 64, 16, 0),
+    ([260], [9000], 2, 1, 64, 0, 0),
+    ([50], [20000], 2, 1, 128, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,klens,heads,kv,d,top,pad", ATTEND)
+def test_block_attention(ctx, lens, klens, heads, kv, d, top, pad, dt):
+    kl = klens or lens
+    q = strided((sum(lens), heads * d), 1, DT[dt], pad)
+    k = strided((sum(kl), kv * d), 2, DT[dt], pad)
+    v = strided((sum(kl), kv * d), 3, DT[dt], pad)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens) if klens else None)
+    sel = lists(plan, heads, top, lens, kl, 4) if top else None
+    out = torch.full((sum(lens), heads * d + pad), 7.0, dtype=DT[dt], device="cuda")
+    ctx.block_attention(plan, q, k, v, heads, kv, out[:, :heads * d], sel=sel)
+    ctx.check()
+    check(out[:, :heads * d], q, k, v, lens, kl, heads, kv, d ** -0.5, sel)
+    assert (out[:, heads * d:] == 7.0).all()
+
+
+@pytest.mark.parametrize("top", [0, 12])
+@pytest.mark.parametrize("scale,size", [(1.0, 3.0), (0.001, 1.0), (4.0, 3.0), (1e-4, 0.1)])
+def test_attention_peaked_and_flat(ctx, scale, size, top):
+    """Scores hundreds apart (the maximum keeps growing, weights underflow) and almost equal ones."""
+    n, heads, d = 1200, 2, 64
+    q, k, v = (randn((n, heads * d), s, torch.bfloat16, size) for s in (1, 2, 3))
+    k *= torch.linspace(0.1, 2.0, n, device="cuda")[:, None].to(torch.bfloat16)  # later keys reach higher
+    plan = ctx.attn_plan([0, n])
+    sel = lists(plan, heads, top, [n], [n], 4) if top else None
+    out = torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, heads, heads, out, scale=scale, sel=sel)
+    check(out, q, k, v, [n], [n], heads, heads, scale, sel)
+
+
+def test_attention_leaves_other_rows(ctx):
+    """Sequences that begin after row 0 and end before the last: the other rows stay, whatever the inputs hold there."""
+    heads, d, lens = 2, 64, [100, 0, 90, 200]
+    q, k, v = (randn((500, heads * d), s, torch.bfloat16) for s in (1, 2, 3))
+    for x in (q, k, v):
+        x[:30] = float("nan")
+        x[30 + sum(lens):] = float("inf")
+    plan = ctx.attn_plan(offsets(lens, 30))
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, heads, out)
+    inner = slice(30, 30 + sum(lens))
+    check(out[inner], q[inner], k[inner], v[inner], lens, lens, heads, heads, d ** -0.5)
+    assert (out[:30] == 7.0).all() and (out[inner.stop:] == 7.0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 3.0e38])
+def test_attention_ignores_what_it_does_not_attend_to(ctx, bad, d):
+    """NaN, infinities and the type's largest values in the neighbouring sequences and in blocks not listed."""
+    heads, lens = 2, [70, 200, 130]
+    q, k, v = (randn((400, heads * d), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan(offsets(lens))
+    sel = torch.full((plan.q_blocks, heads, 2), -1, dtype=torch.int32, device="cuda")
+    sel[1:3, :, 1] = 3  # the middle sequence's short last block (8 rows), listed alone
+    mid = slice(70, 270)
+    clean = [x.clone() for x in (q, k, v)]
+    k[:70], k[270:], v[:70], v[270:] = bad, bad, bad, bad
+    k[70:70 + 192], v[70:70 + 192] = bad, bad
+    out = torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, heads, heads, out, sel=sel)
+    full = torch.full((2, heads, 1), 3)
+    check(out[mid], clean[0][mid], clean[1][mid], clean[2][mid], [200], [200], heads, heads, d ** -0.5, full)
+    assert (out[:70] == 0).all() and (out[270:] == 0).all()  # nothing listed
+
+
+def test_attention_passes_nan_and_infinity_on(ctx):
+    """A NaN score makes its row NaN and no other; a value row's infinity shows where its weight is not 0."""
+    n, d = 300, 64
+    q, k, v = (randn((n, d), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan([0, n])
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, 1, 1, ref)
+    for row in (0, 127, 200):
+        q2 = q.clone()
+        q2[row, 5] = float("nan")
+        ctx.block_attention(plan, q2, k, v, 1, 1, out)
+        assert out[row].isnan().all()
+        out[row] = ref[row]
+        assert torch.equal(out, ref)
+    for col in range(0, n, 7):
+        k2 = k.clone()
+        k2[col, 3] = float("nan")
+        ctx.block_attention(plan, q, k2, v, 1, 1, out)
+        assert out.isnan().all(), col
+    v2 = v.clone()
+    v2[299, 9] = float("inf")
+    ctx.block_attention(plan, q, k, v2, 1, 1, out)
+    assert (out[:, 9] == float("inf")).all()
+    out[:, 9] = ref[:, 9]
+    assert torch.equal(out, ref)
+
+
+def test_attention_of_minus_infinity_scores_is_zero(ctx):
+    n, d = 130, 64
+    q = torch.ones((n, d), dtype=torch.bfloat16, device="cuda")
+    k, v = torch.full_like(q, -float("inf")), randn((n, d), 3, torch.bfloat16)
+    plan = ctx.attn_plan([0, n])
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, 1, 1, out)
+    assert (out == 0).all()
+    k[77] = 0.25  # one key left
+    ctx.block_attention(plan, q, k, v, 1, 1, out)
+    assert torch.equal(out, v[77].expand_as(out))
+
+
+def test_attention_counts_a_block_as_often_as_it_is_listed(ctx):
+    n, d = 256, 64
+    q, k, v = (randn((n, d), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan([0, n])
+    sel = torch.tensor([2, 2, -1, 0, 2], dtype=torch.int32, device="cuda").expand(2, 1, 5).contiguous()
+    out = torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, 1, 1, out, sel=sel)
+    check(out, q, k, v, [n], [n], 1, 1, d ** -0.5, sel)
+
+
+def test_attention_reports_a_block_that_is_not_there(ctx):
+    n, d = 256, 64
+    q, k, v = (randn((n, d), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan([0, n])
+    good = torch.tensor([1, 3, -1], dtype=torch.int32, device="cuda").expand(2, 1, 3).contiguous()
+    out, ref = torch.empty_like(q), torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, 1, 1, ref, sel=good)
+    ctx.check()
+    for wrong in (4, 1 << 30, 2 ** 31 - 1):
+        sel = good.clone()
+        sel[1, 0, 2] = wrong
+        ctx.block_attention(plan, q, k, v, 1, 1, out, sel=sel)
+        with pytest.raises(s3dsp.S3dError):
+            ctx.check()
+        assert torch.equal(out, ref)  # skipped
+        ctx.check()
+
+
+def test_attention_is_deterministic_and_plans_are_reusable(ctx):
+    lens = [1111, 30, 2049]
+    n = sum(lens)
+    q, k, v = (randn((n, 256), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan(offsets(lens))
+    sel = lists(plan, 4, 6, lens, lens, 1)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    for s in (sel, None):
+        ctx.block_attention(plan, q, k, v, 4, 4, a, sel=s)
+        for _ in range(3):
+            ctx.block_attention(plan, q, k, v, 4, 4, b, sel=s)
+            assert torch.equal(a, b)
+
+
+def test_empty_calls(ctx):
+    plan = ctx.attn_plan([0, 0, 0])
+    x = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
+    assert plan.q_blocks == 0 and plan.k_blocks == 0
+    ctx.block_attention(plan, x, x, x, 1, 1, x)
+    ctx.block_select(plan, x, x, 1, 1, torch.empty((0, 1, 4), dtype=torch.int32, device="cuda"))
+    ctx.attn_plan([0])
+    # queries without a single key row anywhere: zeros
+    plan = ctx.attn_plan([0, 70, 300], [0, 0, 0])
+    q = randn((300, 64), 1, torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, x, x, 1, 1, out)
+    assert (out == 0).all()
+    sel = torch.full((plan.q_blocks, 1, 3), 9, dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, x, 1, 1, sel)
+    assert (sel == -1).all()
+    out.fill_(7.0)
+    ctx.block_attention(plan, q, x, x, 1, 1, out, sel=sel)
+    assert (out == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------------
+# streams, graphs, contexts
+# ---------------------------------------------------------------------------------------------------
+def _chain(c, plan, qkv, pos, gq, gk, buf, heads, d):
+    """Norms and rotation out of one projection's rows, selection, attention."""
+    w = heads * d
+    c.qk_norm_rope(qkv[:, :w], heads, gq, buf["q"], qkv[:, w:2 * w], heads, gk, buf["k"], positions=pos,
+                   axis_pairs=[d // 6] * 3)
+    c.block_select(plan, buf["q"], buf["k"], heads, heads, buf["sel"], keep_local=True)
+    c.block_attention(plan, buf["q"], buf["k"], qkv[:, 2 * w:], heads, heads, buf["out"], sel=buf["sel"])
+    c.block_attention(plan, buf["q"][:], buf["k"], qkv[:, 2 * w:], heads, heads, buf["dense"])
+
+
+def _chain_data(lens, heads, d, top, seed, plan):
+    n, w = sum(lens), heads * d
+    new = lambda: torch.full((n, w), 7.0, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    return (randn((n, 3 * w), seed, torch.bfloat16), torch.randint(0, 64, (n, 4), device="cuda", dtype=torch.int32)[:, 1:],
+            randn((heads, d), seed + 1) * 0.1 + 1, randn((heads, d), seed + 2) * 0.1 + 1,
+            dict(q=new(), k=new(), out=new(), dense=new(),
+                 sel=torch.empty((plan.q_blocks, heads, top), dtype=torch.int32, device="cuda")))
+
+
+def test_two_captured_graphs_and_an_eager_call(ctx):
+    """Two graphs captured on one context and replayed on two streams at once, an eager call beside them."""
+    heads, d, top, lens = 4, 64, 4, [900, 33, 1500]
+    stream = torch.cuda.Stream()
+    side = torch.cuda.Stream()
+    c = s3dsp.Context(0, stream=stream.cuda_stream, flags=s3dsp.CONTEXT_DEFERRED_CHECKS)
+    plan = c.attn_plan(offsets(lens))
+    data = [_chain_data(lens, heads, d, top, s, plan) for s in (10, 20, 30)]
+    torch.cuda.synchronize()
+    want = []
+    for x in data:
+        _chain(c, plan, *x, heads, d)
+        stream.synchronize()
+        want.append({k: t.clone() for k, t in x[4].items()})
+        for t in x[4].values():
+            t.fill_(5)
+    torch.cuda.synchronize()
+    graphs = []
+    for x in data[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            _chain(c, plan, *x, heads, d)
+        graphs.append(g)
+    for x in data:
+        for t in x[4].values():
+            t.fill_(5)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        with torch.cuda.stream(stream):
+            graphs[1].replay()
+            _chain(c, plan, *data[2], heads, d)
+    torch.cuda.synchronize()
+    for x, w in zip(data, want):
+        for name, t in w.items():
+            assert torch.equal(x[4][name], t), name
+    c.check()
+
+
+def test_a_plan_is_not_made_inside_a_capture():
+    stream = torch.cuda.Stream()
+    c = s3dsp.Context(0, stream=stream.cuda_stream)
+    x = torch.zeros(16, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        x += 1
+        with pytest.raises(s3dsp.S3dError, match="capture"):
+            c.attn_plan([0, 100])
+    g.replay()
+    torch.cuda.synchronize()
+    assert (x == 1).all()
+
+
+def test_contexts_on_their_own_streams(ctx):
+    """Several contexts at once, each on its own stream, on inputs of their own."""
+    heads, d, top = 2, 64, 3
+    runs = []
+    torch.cuda.synchronize()
+    for s, lens in enumerate(([700], [5, 2000], [1, 1, 1, 400], [1300])):
+        c = s3dsp.Context(0, stream=0, flags=s3dsp.CONTEXT_OWN_STREAM)
+        plan = c.attn_plan(offsets(lens))
+        runs.append((c, plan, _chain_data(lens, heads, d, top, 50 + s, plan), lens))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, plan, x, _ in runs:
+            _chain(c, plan, *x, heads, d)
+    for c, *_ in runs:
+        c.check()
+    for c, plan, x, lens in runs:
+        ref = _chain_data(lens, heads, d, top, 0, plan)[4]
+        plan2 = ctx.attn_plan(offsets(lens))
+        _chain(ctx, plan2, *x[:4], ref, heads, d)
+        torch.cuda.synchronize()
+        for name, t in ref.items():
+            assert torch.equal(x[4][name], t), name
+
+
+def test_sm_limit_changes_nothing(ctx):
+    c = s3dsp.Context(0)
+    c.set_sm_limit(4)
+    lens, heads, d = [300, 1], 2, 64
+    plan = c.attn_plan(offsets(lens), [0, 4000, 9000])
+    q = randn((301, 128), 1, torch.bfloat16)
+    k, v = (randn((9000, 128), s, torch.bfloat16) for s in (2, 3))
+    out = torch.empty_like(q)
+    c.block_attention(plan, q, k, v, heads, heads, out)
+    check(out, q, k, v, lens, [4000, 5000], heads, heads, d ** -0.5)
+
+
+# ---------------------------------------------------------------------------------------------------
+# together: a self-attention layer on the coarse rows of the SLat generator
+# ---------------------------------------------------------------------------------------------------
+def test_together_as_the_middle_of_the_sparse_stages(ctx):
+    """The four operators between the projections (s3dsp_conv), as SlatSparse.forward's `mid` runs them, every
+    step against its definition on the step's own inputs."""
+    coords = np.concatenate([workloads.ellipsoid_shell(24, 0), workloads.ellipsoid_shell(20, 1, batch=1)])
+    dcoords = torch.from_numpy(np.ascontiguousarray(coords)).cuda()
+    heads, d, top = 12, 64, 3
+    w = heads * d
+    h = ctx.hash_build(dcoords)
+    tables = ctx.slat_tables(h)
+    nc = tables.nc
+    coarse = torch.empty((nc, 4), dtype=torch.int32, device="cuda")
+    ctx.slat_tables_export(tables, coarse_coords=coarse)
+    lens = torch.bincount(coarse[:, 0].long(), minlength=2).tolist()
+    assert sum(lens) == nc and min(lens) > 300
+    x = randn((nc, w), 1, torch.bfloat16)
+    wp, ref = [], []
+    for s, (cin, cout) in enumerate(((w, 3 * w), (w, w))):
+        wt = randn((cout, cin), 100 + s, scale=cin ** -0.5)
+        dst = torch.empty(ctx.packed_bytes(s3dsp.PREC_BF16, 1, cin, cout), dtype=torch.uint8, device="cuda")
+        ctx.weights_pack(wt, s3dsp.LAYOUT_LINEAR, 1, cin, cout, s3dsp.PREC_BF16, dst)
+        wp.append(dst)
+        ref.append(wt)
+    plan = ctx.attn_plan(offsets(lens))
+    qkv = torch.empty((nc, 3 * w), dtype=torch.bfloat16, device="cuda")
+    ctx.conv(None, 1, s3dsp.PREC_BF16, x, wp[0], None, qkv, 3 * w)
+    _, _, gq, gk, buf = _chain_data(lens, heads, d, top, 9, plan)
+    _chain(ctx, plan, qkv, coarse[:, 1:], gq, gk, buf, heads, d)
+    y = torch.empty((nc, w), dtype=torch.float32, device="cuda")
+    ctx.conv(None, 1, s3dsp.PREC_BF16, buf["out"], wp[1], None, y, w, residual=x)
+    ctx.check()
+    assert float((qkv.double() - x.double() @ ref[0].to(torch.bfloat16).double().T).norm() / qkv.double().norm()) < 1e-2
+    for name, g, src in (("q", gq, qkv[:, :w]), ("k", gk, qkv[:, w:2 * w])):
+        t = src.double().reshape(nc, heads, d)
+        t = (t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * g.double()).reshape(nc, w)
+        want, size = turned(t, coarse[:, 1:], heads, [d // 6] * 3, 1e4, False, False)
+        within(buf[name], want, size * 26 * F32, unit(torch.bfloat16))
+    assert torch.equal(buf["sel"].cpu(), chosen(buf["q"], buf["k"], lens, lens, heads, heads, top, True))
+    v = qkv[:, 2 * w:]
+    check(buf["out"], buf["q"], buf["k"], v, lens, lens, heads, heads, d ** -0.5, buf["sel"])
+    check(buf["dense"], buf["q"], buf["k"], v, lens, lens, heads, heads, d ** -0.5)
+    want = buf["out"].double() @ ref[1].to(torch.bfloat16).double().T + x.double()
+    assert float((y.double() - want).norm() / want.norm()) < 1e-2
