@@ -33,6 +33,10 @@ namespace {
 constexpr int kQ = kAttnQRows, kK = kAttnKRows;
 constexpr int kQPanel = kQ * 128, kKPanel = kK * 128;  // bytes of 64 columns of a Q / K / V tile
 constexpr float kSlack = 8.f;
+#ifndef KPOLY
+#define KPOLY 2
+#endif
+constexpr int kPolyOfEight = KPOLY;
 
 struct AttnParams {
     const int4* q_blocks;
@@ -44,16 +48,29 @@ struct AttnParams {
     uint32_t* status;
 };
 
+// The blocks of a list go to kGroups softmax warpgroups in turn, each with its
+// own running maximum, sum and accumulator, joined at the end; each group has
+// kBufs score buffers.
+//   D = 64: two groups with one buffer (TMEM: 2 x (64 + 64) columns): with two CTAs per SM, four
+//     softmax warps per scheduler hide each other's chain of waits; the exponentials bound it
+//   D = 128: the accumulators leave room for four buffers in all: one group with two, so that the
+//     next scores are ready when a softmax ends; the MMAs bound it
 template <int D>
 struct Cfg {
     static constexpr int kPanels = D / 64;
+    static constexpr int kGroups = D == 64 ? 2 : 1, kBufs = D == 64 ? 1 : 2;
     static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;  // ring depths: two CTAs per SM
-    static constexpr int kThreads = 128 + 64;
-    static constexpr int kTmemCols = 256;  // S0 64 | S1 64 | O D
-    static constexpr int kOCol = 128;
-    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 2 + 2 + 1 + 1;
+    static constexpr int kSoftmaxWarps = 4 * kGroups;
+    static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+    static constexpr int kGroupCols = 64 * kBufs + D;  // S buffers | O
+    static constexpr int kTmemCols = 256;
+    static_assert(kGroups * kGroupCols == kTmemCols, "TMEM");
+    static constexpr int kOCol = 64 * kBufs;
+    // q_full | k_full, k_empty [kKS] | v_full, v_empty [kVS] | s_full, p_full, o_done [kGroups][kBufs] | drained
+    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 3 * kGroups * kBufs + 1;
     static constexpr size_t kTiles = (size_t)kPanels * kQPanel + (size_t)(kKS + kVS) * kPanels * kKPanel;
-    static constexpr size_t smem(int list) { return 1024 + kTiles + kBars * 8 + 16 + (size_t)list * 4; }
+    static constexpr int kExchange = kGroups > 1 ? kGroups * kQ * 8 : 0;  // (m, l) of each group's rows
+    static constexpr size_t smem(int list) { return 1024 + kTiles + kExchange + kBars * 8 + 16 + (size_t)list * 4; }
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -122,6 +139,55 @@ __device__ __forceinline__ float exp2_hw(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two-lane f32 arithmetic (sm_100: one instruction for both, each rounded as the scalar one)
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ F2 fma2v(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ F2 add2v(F2 a, F2 b) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
+// 2^x on the FMA and integer pipes, for x <= kSlack: x = n + f with n the
+// nearest whole number (read off the low bits of x + 1.5 * 2^23), a minimax
+// polynomial of 2^f on [-1/2, 1/2] (Remez exchange on the relative error:
+// 7.5e-5 of degree 3, far below bf16's rounding of the weight; 2.7e-6 of degree
+// 4 for f16), and n added to the exponent. x below -126 counts as -126.
+template <bool kF16>
+__device__ __forceinline__ F2 exp2_poly(F2 x) {
+    constexpr float kMagic = 12582912.f;
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const F2 t = add2v(x, both(kMagic));
+    const F2 f = add2v(x, fma2v(add2v(t, both(-kMagic)), both(-1.f), both(0.f)));
+    F2 p;
+    if constexpr (kF16) {
+        p = fma2v(both(0.009570102207362652f), f, both(0.05591785907745361f));
+        p = fma2v(p, f, both(0.240247443318367f));
+        p = fma2v(p, f, both(0.6931217908859253f));
+        p = fma2v(p, f, both(0.9999992847442627f));
+    } else {
+        p = fma2v(both(0.0551716685295105f), f, both(0.2426111251115799f));
+        p = fma2v(p, f, both(0.6932609677314758f));
+        p = fma2v(p, f, both(0.9999280571937561f));
+    }
+    return F2{__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+              __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23))};
+}
 // (lo, hi) as two 16-bit floats of one register
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -138,15 +204,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     block_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                            const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
     using C = Cfg<D>;
+    constexpr int G = C::kGroups, B = C::kBufs;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* sm = raw + (base - smem_u32(raw));
     const uint32_t sQ = base, sK = sQ + C::kPanels * kQPanel, sV = sK + C::kKS * C::kPanels * kKPanel;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles);
-    const uint32_t b0 = smem_u32(bars);
-    const uint32_t q_full = b0, k_full = b0 + 8, k_empty = k_full + 8 * C::kKS, v_full = k_empty + 8 * C::kKS,
-                   v_empty = v_full + 8 * C::kVS, s_full = v_empty + 8 * C::kVS, p_full = s_full + 16,
-                   o_done = p_full + 16, drained = o_done + 8;
+    float2* exchange = reinterpret_cast<float2*>(sm + C::kTiles);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles + C::kExchange);
+    const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, k_empty = k_full + 8 * C::kKS,
+                   v_full = k_empty + 8 * C::kKS, v_empty = v_full + 8 * C::kVS, s_full = v_empty + 8 * C::kVS,
+                   p_full = s_full + 8 * G * B, o_done = p_full + 8 * G * B, drained = o_done + 8 * G * B;
     volatile int* abort_flag = reinterpret_cast<int*>(bars + C::kBars);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + C::kBars) + 1;
     volatile int* n_listed = reinterpret_cast<int*>(bars + C::kBars) + 2;
@@ -154,13 +221,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     int* list = reinterpret_cast<int*>(bars + C::kBars) + 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProdWarp = 4, kMmaWarp = 5;
+    constexpr int kProdWarp = C::kSoftmaxWarps, kMmaWarp = C::kSoftmaxWarps + 1;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < C::kKS; ++s) mbar_init(k_full + 8 * s, 1), mbar_init(k_empty + 8 * s, 1);
         for (int s = 0; s < C::kVS; ++s) mbar_init(v_full + 8 * s, 1), mbar_init(v_empty + 8 * s, 1);
-        for (int s = 0; s < 2; ++s) mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, kQ);
-        mbar_init(o_done, 1);
+        for (int s = 0; s < G * B; ++s)
+            mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4), mbar_init(o_done + 8 * s, 1);
         mbar_init(drained, 1);
         *abort_flag = 0;
         *drain_flag = 0;
@@ -244,48 +311,54 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         constexpr uint32_t kIdescPV = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) |
                                       ((kQ >> 4) << 24);
         constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
-        bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag, p.status);
+        // all lanes leave a wait together: none is left behind by more than a phase
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status)) != 0;
+        };
+        bool ok = n == 0 || wait(q_full, 0);
         auto qk = [&](int j) {
-            const int s = j % C::kKS;
-            if (!mbar_wait(k_full + 8 * s, (j / C::kKS) & 1, abort_flag, p.status)) return false;
+            const int s = j % C::kKS, g = j % G, b = (j / G) % B;
+            if (!wait(k_full + 8 * s, (j / C::kKS) & 1)) return false;
             tc_fence_after();
             if (lane == 0) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
-                    mma_bf16(tmem + 64 * (j & 1), sw128_desc(sQ + (ks / 4) * kQPanel + (ks % 4) * 32),
+                    mma_bf16(tmem + g * C::kGroupCols + 64 * b, sw128_desc(sQ + (ks / 4) * kQPanel + (ks % 4) * 32),
                              sw128_desc(sK + s * kTileBytes + (ks / 4) * kKPanel + (ks % 4) * 32), kIdescQK, ks > 0);
-                mma_commit(s_full + 8 * (j & 1));
+                mma_commit(s_full + 8 * (g * B + b));
                 mma_commit(k_empty + 8 * s);
             }
             return true;
         };
-        for (int j = 0; j < min(n, 2) && ok; ++j) ok = qk(j);
+        for (int j = 0; j < min(n, G * B) && ok; ++j) ok = qk(j);
         for (int j = 0; j < n && ok; ++j) {
-            const int t = j % C::kVS;
+            const int t = j % C::kVS, g = j % G, i = j / G, b = i % B;
             const uint32_t v0 = sV + t * kTileBytes;
-            ok = mbar_wait(v_full + 8 * t, (j / C::kVS) & 1, abort_flag, p.status);
+            ok = wait(v_full + 8 * t, (j / C::kVS) & 1);
             if (!ok) break;
             const int rows = rows_of(block_of(j));
             if (rows < kK) {
                 // V rows that are not the sequence's: zeros (p is 0 there, and 0 * NaN is not)
-                for (int i = 0; i < C::kPanels; ++i)
+                for (int x = 0; x < C::kPanels; ++x)
                     for (uint32_t a = rows * 128 + lane * 16; a < (uint32_t)kKPanel; a += 32 * 16)
-                        *reinterpret_cast<uint4*>(sm + (v0 - base) + i * kKPanel + a) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sm + (v0 - base) + x * kKPanel + a) = make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             }
-            ok = mbar_wait(p_full + 8 * (j & 1), (j >> 1) & 1, abort_flag, p.status);
+            ok = wait(p_full + 8 * (g * B + b), (i / B) & 1);
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
+                const uint32_t tg = tmem + g * C::kGroupCols;
 #pragma unroll
                 for (int ks = 0; ks < kK / 16; ++ks)
-                    mma_ts(tmem + C::kOCol, tmem + 64 * (j & 1) + 8 * ks, mn_desc(v0 + ks * 2048), kIdescPV,
-                           (j > 0 || ks > 0) ? 1u : 0u);
-                mma_commit(o_done);
+                    mma_ts(tg + C::kOCol, tg + 64 * b + 8 * ks, mn_desc(v0 + ks * 2048), kIdescPV,
+                           (i > 0 || ks > 0) ? 1u : 0u);
+                mma_commit(o_done + 8 * (g * B + b));
                 mma_commit(v_empty + 8 * t);
             }
-            if (j + 2 < n) ok = mbar_wait(o_done, j & 1, abort_flag, p.status) && qk(j + 2);
+            // the next scores of this buffer, once its weights have been read
+            if (j + G * B < n) ok = wait(o_done + 8 * (g * B + b), (i / B) & 1) && qk(j + G * B);
         }
         __syncwarp();
         if (!__all_sync(0xffffffffu, ok)) {
@@ -296,113 +369,161 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             }
         }
     } else {
-        // ================= softmax: thread = query row (TMEM lane) =================
-        const int row = threadIdx.x;
-        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
-        const bool live = 32 * warp < q_rows;  // a warp without rows only keeps the barriers' counts
+        // ================= softmax: thread = query row (TMEM lane) of one group =================
+        const int g = warp / 4, row = threadIdx.x & (kQ - 1);
+        const uint32_t tg = tmem + g * C::kGroupCols + ((uint32_t)(32 * (warp & 3)) << 16);
+        const bool live = 32 * (warp & 3) < q_rows;  // a warp without rows only keeps the barriers' counts
+        const int ng = (n - g + G - 1) / G;          // this group's blocks
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            const uint32_t ts = lane_base + 64 * (j & 1);
-            ok = mbar_wait(s_full + 8 * (j & 1), (j >> 1) & 1, abort_flag, p.status);
+        for (int i = 0; i < ng; ++i) {
+            const int b = i % B;
+            const uint32_t ts = tg + 64 * b;
+            ok = mbar_wait(s_full + 8 * (g * B + b), (i / B) & 1, abort_flag, p.status);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             if (live) {
-                uint32_t s[2][32];
-                tmem_ld32(ts, s[0]);
-                tmem_ld32(ts + 32, s[1]);
-                tmem_wait_ld();
-                tmem_settle(s[0]);
-                tmem_settle(s[1]);
-                const int rows = rows_of(block_of(j));
-                if (rows < kK) {
+                const int rows = rows_of(block_of(i * G + g));
+                uint32_t s[32];
+                float mx[4] = {m, m, m, m};
 #pragma unroll
-                    for (int i = 0; i < kK; ++i)
-                        if (i >= rows) s[i / 32][i % 32] = 0xff800000u;  // -inf
+                for (int half = 1; half >= 0; --half) {
+                    tmem_ld32(ts + 32 * half, s);
+                    tmem_wait_ld();
+                    tmem_settle(s);
+                    if (rows < kK) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (32 * half + x >= rows) s[x] = 0xff800000u;  // -inf
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2)
+                        mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
                 }
-                float mx = m;
-#pragma unroll
-                for (int i = 0; i < kK; i += 2)
-                    mx = max3(mx, __uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
+                const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
                 // a NaN maximum always counts as grown, and stays
-                const bool grown = !((mx - m) * p.c <= kSlack) && !(mx == -INFINITY);
+                const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float to = grown ? mx : m;
+                    const float to = grown ? mt : m;
                     const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
-                    if (j > 0) {
-                        ok = mbar_wait(o_done, (j - 1) & 1, abort_flag, p.status);
+                    if (i > 0) {
+                        ok = mbar_wait(o_done + 8 * (g * B + (i - 1) % B), ((i - 1) / B) & 1, abort_flag, p.status);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (int c0 = 0; c0 < D; c0 += 32) {
                             uint32_t o[32];
-                            tmem_ld32(lane_base + C::kOCol + c0, o);
+                            tmem_ld32(tg + C::kOCol + c0, o);
                             tmem_wait_ld();
                             tmem_settle(o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st32(lane_base + C::kOCol + c0, o);
+                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                            tmem_st32(tg + C::kOCol + c0, o);
                         }
                     }
                     l *= alpha;
                     m = to;
                 }
-                const float bias = m == -INFINITY ? 0.f : -m * p.c;
-                float sum0 = 0.f, sum1 = 0.f;
+                // an infinite maximum makes its row NaN, as inf - inf does
+                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
+                F2 sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
+                    // the lower half is still in registers (its P overwrites columns 0 .. 15, read for
+                    // good); the upper one is read again, which leaves registers for the other warps
+                    if (half == 1) {
+                        tmem_ld32(ts + 32, s);
+                        tmem_wait_ld();
+                        tmem_settle(s);
+                        if (rows < kK) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x)
+                                if (32 + x >= rows) s[x] = 0xff800000u;
+                        }
+                    }
                     uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float p0 = exp2_hw(fmaf(__uint_as_float(s[half][2 * i]), p.c, bias));
-                        const float p1 = exp2_hw(fmaf(__uint_as_float(s[half][2 * i + 1]), p.c, bias));
-                        sum0 += p0;
-                        sum1 += p1;
-                        w[i] = pack2<kF16>(p0, p1);
+                    for (int x = 0; x < 16; ++x) {
+                        F2 v = fma2v(F2{__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])}, both(p.c), bias);
+                        if ((x & 7) < kPolyOfEight)
+                            v = exp2_poly<kF16>(v);
+                        else
+                            v = F2{exp2_hw(v.x), exp2_hw(v.y)};
+                        sum[x & 1] = add2v(sum[x & 1], v);
+                        w[x] = pack2<kF16>(v.x, v.y);
                     }
                     tmem_st16(ts + 16 * half, w);
                 }
-                l += sum0 + sum1;
+                const F2 both_sums = add2v(sum[0], sum[1]);
+                l += both_sums.x + both_sums.y;
                 tmem_wait_st();
             }
             tc_fence_before();
-            mbar_arrive(p_full + 8 * (j & 1));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * (g * B + b));
         }
-        if (ok && n > 0) {
-            // o_done's phases one by one: a parity says nothing about a phase two back
-            // (s_full(n - 1) was seen, so phase n - 3 is over)
-            ok = (n < 2 || mbar_wait(o_done, n & 1, abort_flag, p.status)) &&
-                 mbar_wait(o_done, (n - 1) & 1, abort_flag, p.status);
+        if (ok && ng > 0) {
+            // the last product (they complete in order). A wait tells two neighbouring phases of its
+            // barrier apart: with one o_done per buffer the phase before is over when s_full is seen
+            ok = mbar_wait(o_done + 8 * (g * B + (ng - 1) % B), ((ng - 1) / B) & 1, abort_flag, p.status);
             ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
         }
+        tc_fence_before();
+        float a[G];  // what each group's accumulator counts for, divided by the sum
+        if constexpr (G > 1) {
+            exchange[g * kQ + row] = make_float2(m, l);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftmaxWarps) : "memory");
+            float2 ml[G];
+            float top = -INFINITY;  // of all groups
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                ml[x] = exchange[x * kQ + row];
+                top = max3(top, ml[x].x, ml[x].x);
+            }
+            l = 0.f;
+#pragma unroll
+            for (int x = 0; x < G; ++x) {
+                a[x] = top == -INFINITY ? 1.f : exp2_hw((ml[x].x - top) * p.c);
+                l = fmaf(a[x], ml[x].y, l);
+            }
+            m = top;
+        } else {
+            a[0] = 1.f;
+        }
+        tc_fence_after();
         if (ok && live) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            // nothing listed, or every score -inf (exp2_poly gives those a weight of 2^-126, not 0)
+            const bool none = m == -INFINITY || l == 0.f;
+            const float inv = none ? 0.f : 1.f / l;
             uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(q_row0 + row) * p.out_stride + (int64_t)h * D;
+            const uint32_t t0 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kOCol;
+            // each group writes its share of the columns
 #pragma unroll
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld32(lane_base + C::kOCol + c0, o);
+            for (int c0 = g * (D / G); c0 < (g + 1) * (D / G); c0 += 32) {
+                float o[32];
+#pragma unroll
+                for (int y = 0; y < 32; ++y) o[y] = 0.f;
+#pragma unroll
+                for (int x = 0; x < G; ++x) {
+                    if (n <= x) break;  // that group had no block: its accumulator was never written
+                    uint32_t v[32];
+                    tmem_ld32(t0 + x * C::kGroupCols + c0, v);
                     tmem_wait_ld();
-                    tmem_settle(o);
-                } else {
+                    tmem_settle(v);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    for (int y = 0; y < 32; ++y) o[y] = fmaf(__uint_as_float(v[y]), a[x] * inv, o[y]);
                 }
                 if (row < q_rows) {
                     uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int y = 0; y < 4; ++y) {
                         uint32_t w[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            w[x] = l == 0.f ? 0u
-                                            : pack2<kF16>(__uint_as_float(o[8 * i + 2 * x]) * inv,
-                                                          __uint_as_float(o[8 * i + 2 * x + 1]) * inv);
-                        d4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                            w[x] = none ? 0u : pack2<kF16>(o[8 * y + 2 * x], o[8 * y + 2 * x + 1]);
+                        d4[y] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
