@@ -9,9 +9,17 @@
 //   softmax warps   one thread per query row: S from TMEM, running maximum, p = 2^(c s - c m),
 //                   running sum, P back into S's columns
 //
-// S is double-buffered: the next block's scores are computed while this
-// block's softmax runs, and P(j) V(j) while softmax(j + 1) runs. A buffer is
-// written by Q K^T(j + 2) only after P(j) V(j), its last reader, has completed.
+// kBufs score buffers: the scores of the next blocks are computed while this
+// block's softmax runs, and P(j) V(j) while softmax(j + 1) runs, so that the
+// softmax warps wait for neither. P(j) takes the first columns of S(j); Q K^T
+// writes a buffer again only after P V, its last reader, has completed.
+//
+// What bounds it (one B200; us per 128 x 64 tile and SM, dense 4096^2 rows):
+//   d = 64   0.434 (715 TFLOP/s): without the exponentials 0.34, without MMAs 0.40, MMAs and barriers
+//            alone 0.29. Two softmax warps per scheduler issue in 54 % of the cycles, the tensor pipe is
+//            busy in 48 %: the chain of a softmax step (score load, maximum, exponentials, P store). More
+//            warps did not help: two groups or two threads per row, or four CTAs per SM, took 0.44 - 0.51.
+//   d = 128  0.517 (1,200 TFLOP/s, 0.71 of the measured bf16 peak): MMAs and barriers alone 0.45
 //
 // The accumulator is rescaled only when a row's maximum has grown by more than
 // kSlack (in powers of two) over the one in use: the softmax is the same for
@@ -33,10 +41,10 @@ namespace {
 constexpr int kQ = kAttnQRows, kK = kAttnKRows;
 constexpr int kQPanel = kQ * 128, kKPanel = kK * 128;  // bytes of 64 columns of a Q / K / V tile
 constexpr float kSlack = 8.f;
-#ifndef KPOLY
-#define KPOLY 2
-#endif
-constexpr int kPolyOfEight = KPOLY;
+// pairs of eight whose exponentials go to the FMA pipe (exp2_poly) instead of
+// the special-function unit, which gives 16 a cycle and SM: at d = 64, 4096^2
+// rows x 148 heads, 0 / 1 / 2 / 3 of eight took 910 / 903 / 893 / 960 us
+constexpr int kPolyOfEight = 2;
 
 struct AttnParams {
     const int4* q_blocks;
@@ -48,31 +56,44 @@ struct AttnParams {
     uint32_t* status;
 };
 
-// The blocks of a list go to kGroups softmax warpgroups in turn, each with its
-// own running maximum, sum and accumulator, joined at the end; each group has
-// kBufs score buffers.
-//   D = 64: two groups with one buffer (TMEM: 2 x (64 + 64) columns): with two CTAs per SM, four
-//     softmax warps per scheduler hide each other's chain of waits; the exponentials bound it
-//   D = 128: the accumulators leave room for four buffers in all: one group with two, so that the
-//     next scores are ready when a softmax ends; the MMAs bound it
+// Two CTAs per SM: 256 of its 512 TMEM columns each, kBufs score buffers of 64
+// columns and the accumulator; K and V rings as deep as half the shared memory
+// takes.
 template <int D>
 struct Cfg {
     static constexpr int kPanels = D / 64;
-    static constexpr int kGroups = D == 64 ? 2 : 1, kBufs = D == 64 ? 1 : 2;
-    static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;  // ring depths: two CTAs per SM
-    static constexpr int kSoftmaxWarps = 4 * kGroups;
-    static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
-    static constexpr int kGroupCols = 64 * kBufs + D;  // S buffers | O
+    static constexpr int kBufs = D == 64 ? 3 : 2;  // blocks whose scores are computed ahead of the softmax
+    static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;
+    static constexpr int kThreads = 128 + 64;
     static constexpr int kTmemCols = 256;
-    static_assert(kGroups * kGroupCols == kTmemCols, "TMEM");
-    static constexpr int kOCol = 64 * kBufs;
-    // q_full | k_full, k_empty [kKS] | v_full, v_empty [kVS] | s_full, p_full, o_done [kGroups][kBufs] | drained
-    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 3 * kGroups * kBufs + 1;
+    static constexpr int kOCol = 64 * kBufs;  // S buffers | O
+    static_assert(kOCol + D == kTmemCols, "TMEM");
+    // q_full | k_full, k_empty [kKS] | v_full, v_empty [kVS] | s_full, p_full, o_done [kBufs] | drained
+    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 3 * kBufs + 1;
     static constexpr size_t kTiles = (size_t)kPanels * kQPanel + (size_t)(kKS + kVS) * kPanels * kKPanel;
-    static constexpr int kExchange = kGroups > 1 ? kGroups * kQ * 8 : 0;  // (m, l) of each group's rows
-    static constexpr size_t smem(int list) { return 1024 + kTiles + kExchange + kBars * 8 + 16 + (size_t)list * 4; }
+    static constexpr size_t smem(int list) { return 1024 + kTiles + kBars * 8 + 16 + (size_t)list * 4; }
 };
 
+
+// A place in a ring of N: the slot and the parity of its current pass.
+template <int N>
+struct Cursor {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) slot = 0, parity ^= 1u;
+    }
+};
+
+// true in one lane of the (converged) warp. The compiler knows that a branch
+// on it has one thread, so MMA descriptors stay in uniform registers: behind
+// `lane == 0` each tcgen05 instruction cost about 80 cycles to issue, which
+// made the issuing warp the bottleneck.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -107,12 +128,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::S3DSP_I8(v, 0),
-        S3DSP_I8(v, 8), S3DSP_I8(v, 16), S3DSP_I8(v, 24), "r"(taddr)
-        : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::S3DSP_I8(v, 0), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// values loaded by tmem_ld32, usable only from here on: the compiler sees them
+// change after the wait, so no use moves before it
+__device__ __forceinline__ void tmem_settle(uint32_t (&v)[32]) {
+    asm volatile("" : S3DSP_RW8(v, 0), S3DSP_RW8(v, 8), S3DSP_RW8(v, 16), S3DSP_RW8(v, 24)::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -121,11 +145,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         S3DSP_I8(v, 8), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// values loaded by tmem_ld32, usable only from here on: the compiler sees them
-// change after the wait, so no use moves before it
-__device__ __forceinline__ void tmem_settle(uint32_t (&v)[32]) {
-    asm volatile("" : S3DSP_RW8(v, 0), S3DSP_RW8(v, 8), S3DSP_RW8(v, 16), S3DSP_RW8(v, 24)::"memory");
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : S3DSP_R8(v, 0) : "r"(taddr) : "memory");
+    tmem_wait_ld();
+    asm volatile("" : S3DSP_RW8(v, 0)::"memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // the larger of three; NaN if one is
@@ -204,16 +227,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     block_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                            const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
     using C = Cfg<D>;
-    constexpr int G = C::kGroups, B = C::kBufs;
+    constexpr int B = C::kBufs;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* sm = raw + (base - smem_u32(raw));
     const uint32_t sQ = base, sK = sQ + C::kPanels * kQPanel, sV = sK + C::kKS * C::kPanels * kKPanel;
-    float2* exchange = reinterpret_cast<float2*>(sm + C::kTiles);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles + C::kExchange);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles);
     const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, k_empty = k_full + 8 * C::kKS,
                    v_full = k_empty + 8 * C::kKS, v_empty = v_full + 8 * C::kVS, s_full = v_empty + 8 * C::kVS,
-                   p_full = s_full + 8 * G * B, o_done = p_full + 8 * G * B, drained = o_done + 8 * G * B;
+                   p_full = s_full + 8 * B, o_done = p_full + 8 * B, drained = o_done + 8 * B;
     volatile int* abort_flag = reinterpret_cast<int*>(bars + C::kBars);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + C::kBars) + 1;
     volatile int* n_listed = reinterpret_cast<int*>(bars + C::kBars) + 2;
@@ -221,12 +243,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     int* list = reinterpret_cast<int*>(bars + C::kBars) + 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProdWarp = C::kSoftmaxWarps, kMmaWarp = C::kSoftmaxWarps + 1;
+    constexpr int kProdWarp = 4, kMmaWarp = 5;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         for (int s = 0; s < C::kKS; ++s) mbar_init(k_full + 8 * s, 1), mbar_init(k_empty + 8 * s, 1);
         for (int s = 0; s < C::kVS; ++s) mbar_init(v_full + 8 * s, 1), mbar_init(v_empty + 8 * s, 1);
-        for (int s = 0; s < G * B; ++s)
+        for (int s = 0; s < B; ++s)
             mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4), mbar_init(o_done + 8 * s, 1);
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -271,27 +293,28 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
 
     if (warp == kProdWarp) {
         // ================= TMA producer =================
-        if (lane == 0 && n > 0) {
+        if (n > 0 && elect_one()) {
             constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
             const int qc = h * D, kc = (h / p.per_kv) * D;
             mbar_arrive_tx(q_full, C::kPanels * kQPanel);
             for (int i = 0; i < C::kPanels; ++i) tma_load_2d(sQ + i * kQPanel, &qmap, qc + 64 * i, q_row0, q_full);
             int issued_k = 0, issued_v = 0;
             bool ok = true;
-            for (int j = 0; j < n && ok; ++j) {
+            Cursor<C::kKS> ks;
+            Cursor<C::kVS> vs;
+            for (int j = 0; j < n && ok; ++j, ks.next(), vs.next()) {
                 const int y = k_row0 + block_of(j) * kK;
-                const int s = j % C::kKS, t = j % C::kVS;
-                ok = mbar_wait(k_empty + 8 * s, ((j / C::kKS) & 1) ^ 1, abort_flag, p.status);
+                ok = mbar_wait(k_empty + 8 * ks.slot, ks.parity ^ 1u, abort_flag, p.status);
                 if (!ok) break;
-                mbar_arrive_tx(k_full + 8 * s, kTileBytes);
+                mbar_arrive_tx(k_full + 8 * ks.slot, kTileBytes);
                 for (int i = 0; i < C::kPanels; ++i)
-                    tma_load_2d(sK + s * kTileBytes + i * kKPanel, &kmap, kc + 64 * i, y, k_full + 8 * s);
+                    tma_load_2d(sK + ks.slot * kTileBytes + i * kKPanel, &kmap, kc + 64 * i, y, k_full + 8 * ks.slot);
                 ++issued_k;
-                ok = mbar_wait(v_empty + 8 * t, ((j / C::kVS) & 1) ^ 1, abort_flag, p.status);
+                ok = mbar_wait(v_empty + 8 * vs.slot, vs.parity ^ 1u, abort_flag, p.status);
                 if (!ok) break;
-                mbar_arrive_tx(v_full + 8 * t, kTileBytes);
+                mbar_arrive_tx(v_full + 8 * vs.slot, kTileBytes);
                 for (int i = 0; i < C::kPanels; ++i)
-                    tma_load_2d(sV + t * kTileBytes + i * kKPanel, &vmap, kc + 64 * i, y, v_full + 8 * t);
+                    tma_load_2d(sV + vs.slot * kTileBytes + i * kKPanel, &vmap, kc + 64 * i, y, v_full + 8 * vs.slot);
                 ++issued_v;
             }
             if (!ok) {
@@ -305,215 +328,176 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
-        // ================= MMA issuer (the whole warp walks, lane 0 issues) =================
-        constexpr uint32_t kFmt = kF16 ? 0u : 1u;
-        constexpr uint32_t kIdescQK = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kK >> 3) << 17) | ((kQ >> 4) << 24);
-        constexpr uint32_t kIdescPV = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) |
-                                      ((kQ >> 4) << 24);
-        constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
-        // all lanes leave a wait together: none is left behind by more than a phase
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status)) != 0;
-        };
-        bool ok = n == 0 || wait(q_full, 0);
-        auto qk = [&](int j) {
-            const int s = j % C::kKS, g = j % G, b = (j / G) % B;
-            if (!wait(k_full + 8 * s, (j / C::kKS) & 1)) return false;
-            tc_fence_after();
-            if (lane == 0) {
+        // ================= MMA issuer =================
+        if (n > 0 && elect_one()) {
+            constexpr uint32_t kFmt = kF16 ? 0u : 1u;
+            constexpr uint32_t kIdescQK = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kK >> 3) << 17) | ((kQ >> 4) << 24);
+            constexpr uint32_t kIdescPV = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) |
+                                          ((kQ >> 4) << 24);
+            constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
+            auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dv = mn_desc(sV);
+            Cursor<C::kKS> ks;  // the next K tile, score buffer
+            Cursor<B> sb;
+            auto qk = [&]() {
+                if (!wait(k_full + 8 * ks.slot, ks.parity)) return false;
+                tc_fence_after();
+                const uint64_t dkt = dk + ((ks.slot * kTileBytes) >> 4);
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    mma_bf16(tmem + g * C::kGroupCols + 64 * b, sw128_desc(sQ + (ks / 4) * kQPanel + (ks % 4) * 32),
-                             sw128_desc(sK + s * kTileBytes + (ks / 4) * kKPanel + (ks % 4) * 32), kIdescQK, ks > 0);
-                mma_commit(s_full + 8 * (g * B + b));
-                mma_commit(k_empty + 8 * s);
-            }
-            return true;
-        };
-        for (int j = 0; j < min(n, G * B) && ok; ++j) ok = qk(j);
-        for (int j = 0; j < n && ok; ++j) {
-            const int t = j % C::kVS, g = j % G, i = j / G, b = i % B;
-            const uint32_t v0 = sV + t * kTileBytes;
-            ok = wait(v_full + 8 * t, (j / C::kVS) & 1);
-            if (!ok) break;
-            const int rows = rows_of(block_of(j));
-            if (rows < kK) {
-                // V rows that are not the sequence's: zeros (p is 0 there, and 0 * NaN is not)
-                for (int x = 0; x < C::kPanels; ++x)
-                    for (uint32_t a = rows * 128 + lane * 16; a < (uint32_t)kKPanel; a += 32 * 16)
-                        *reinterpret_cast<uint4*>(sm + (v0 - base) + x * kKPanel + a) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
-            ok = wait(p_full + 8 * (g * B + b), (i / B) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            if (lane == 0) {
-                const uint32_t tg = tmem + g * C::kGroupCols;
+                for (int x = 0; x < D / 16; ++x)
+                    mma_bf16(tmem + 64 * sb.slot, dq + (((x / 4) * kQPanel + (x % 4) * 32) >> 4),
+                             dkt + (((x / 4) * kKPanel + (x % 4) * 32) >> 4), kIdescQK, x > 0);
+                mma_commit(s_full + 8 * sb.slot);
+                mma_commit(k_empty + 8 * ks.slot);
+                ks.next();
+                sb.next();
+                return true;
+            };
+            bool ok = wait(q_full, 0);
+            for (int j = 0; j < min(n, B) && ok; ++j) ok = qk();
+            Cursor<C::kVS> vs;
+            Cursor<B> pb;
+            for (int j = 0; j < n && ok; ++j, vs.next(), pb.next()) {
+                ok = wait(v_full + 8 * vs.slot, vs.parity) && wait(p_full + 8 * pb.slot, pb.parity);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t dvt = dv + ((vs.slot * kTileBytes) >> 4);
 #pragma unroll
-                for (int ks = 0; ks < kK / 16; ++ks)
-                    mma_ts(tg + C::kOCol, tg + 64 * b + 8 * ks, mn_desc(v0 + ks * 2048), kIdescPV,
-                           (i > 0 || ks > 0) ? 1u : 0u);
-                mma_commit(o_done + 8 * (g * B + b));
-                mma_commit(v_empty + 8 * t);
+                for (int x = 0; x < kK / 16; ++x)
+                    mma_ts(tmem + C::kOCol, tmem + 64 * pb.slot + 8 * x, dvt + ((x * 2048) >> 4), kIdescPV,
+                           (j > 0 || x > 0) ? 1u : 0u);
+                mma_commit(o_done + 8 * pb.slot);
+                mma_commit(v_empty + 8 * vs.slot);
+                // this buffer's next scores, once its weights have been read
+                if (j + B < n) ok = wait(o_done + 8 * pb.slot, pb.parity) && qk();
             }
-            // the next scores of this buffer, once its weights have been read
-            if (j + G * B < n) ok = wait(o_done + 8 * (g * B + b), (i / B) & 1) && qk(j + G * B);
-        }
-        __syncwarp();
-        if (!__all_sync(0xffffffffu, ok)) {
-            // the MMAs issued so far end before their operands are given back
-            if (lane == 0) {
+            if (!ok) {
+                // the MMAs issued so far end before their operands are given back
                 mma_commit(drained);
                 mbar_wait(drained, 0, drain_flag, p.status);
             }
         }
+        __syncwarp();
     } else {
-        // ================= softmax: thread = query row (TMEM lane) of one group =================
-        const int g = warp / 4, row = threadIdx.x & (kQ - 1);
-        const uint32_t tg = tmem + g * C::kGroupCols + ((uint32_t)(32 * (warp & 3)) << 16);
-        const bool live = 32 * (warp & 3) < q_rows;  // a warp without rows only keeps the barriers' counts
-        const int ng = (n - g + G - 1) / G;          // this group's blocks
+        // ================= softmax: thread = query row (TMEM lane) =================
+        const int row = threadIdx.x;
+        const uint32_t t0 = tmem + ((uint32_t)(32 * warp) << 16);
+        const bool live = 32 * warp < q_rows;  // a warp without rows only keeps the barriers' counts
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int i = 0; i < ng; ++i) {
-            const int b = i % B;
-            const uint32_t ts = tg + 64 * b;
-            ok = mbar_wait(s_full + 8 * (g * B + b), (i / B) & 1, abort_flag, p.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (live) {
-                const int rows = rows_of(block_of(i * G + g));
-                uint32_t s[32];
-                float mx[4] = {m, m, m, m};
-#pragma unroll
-                for (int half = 1; half >= 0; --half) {
-                    tmem_ld32(ts + 32 * half, s);
-                    tmem_wait_ld();
-                    tmem_settle(s);
-                    if (rows < kK) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (32 * half + x >= rows) s[x] = 0xff800000u;  // -inf
-                    }
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2)
-                        mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-                }
-                const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                // a NaN maximum always counts as grown, and stays
-                const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float to = grown ? mt : m;
-                    const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
-                    if (i > 0) {
-                        ok = mbar_wait(o_done + 8 * (g * B + (i - 1) % B), ((i - 1) / B) & 1, abort_flag, p.status);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(tg + C::kOCol + c0, o);
-                            tmem_wait_ld();
-                            tmem_settle(o);
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-                            tmem_st32(tg + C::kOCol + c0, o);
-                        }
-                    }
-                    l *= alpha;
-                    m = to;
-                }
-                // an infinite maximum makes its row NaN, as inf - inf does
-                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
-                F2 sum[2] = {both(0.f), both(0.f)};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    // the lower half is still in registers (its P overwrites columns 0 .. 15, read for
-                    // good); the upper one is read again, which leaves registers for the other warps
-                    if (half == 1) {
-                        tmem_ld32(ts + 32, s);
-                        tmem_wait_ld();
-                        tmem_settle(s);
-                        if (rows < kK) {
-#pragma unroll
-                            for (int x = 0; x < 32; ++x)
-                                if (32 + x >= rows) s[x] = 0xff800000u;
-                        }
-                    }
-                    uint32_t w[16];
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        F2 v = fma2v(F2{__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])}, both(p.c), bias);
-                        if ((x & 7) < kPolyOfEight)
-                            v = exp2_poly<kF16>(v);
-                        else
-                            v = F2{exp2_hw(v.x), exp2_hw(v.y)};
-                        sum[x & 1] = add2v(sum[x & 1], v);
-                        w[x] = pack2<kF16>(v.x, v.y);
-                    }
-                    tmem_st16(ts + 16 * half, w);
-                }
-                const F2 both_sums = add2v(sum[0], sum[1]);
-                l += both_sums.x + both_sums.y;
-                tmem_wait_st();
-            }
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status)) != 0;
+        };
+        Cursor<B> sb, ob;  // the block's buffer, and that of the product before it
+        // V rows of block j that are not the sequence's: zeros (p is 0 there, and 0 * NaN is not)
+        auto clear_tail = [&](int j, int rows) {
+            const int t = j % C::kVS;
+            if (!wait(v_full + 8 * t, (j / C::kVS) & 1)) return false;
+            for (int x = 0; x < C::kPanels; ++x)
+                for (int a = rows * 128 + row * 16; a < kKPanel; a += kQ * 16)
+                    *reinterpret_cast<uint4*>(sm + (sV - base) + (t * C::kPanels + x) * kKPanel + a) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            return true;
+        };
+        auto hand_over = [&]() {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 8 * (g * B + b));
-        }
-        if (ok && ng > 0) {
-            // the last product (they complete in order). A wait tells two neighbouring phases of its
-            // barrier apart: with one o_done per buffer the phase before is over when s_full is seen
-            ok = mbar_wait(o_done + 8 * (g * B + (ng - 1) % B), ((ng - 1) / B) & 1, abort_flag, p.status);
-            ok = __all_sync(0xffffffffu, ok);
-        }
-        tc_fence_before();
-        float a[G];  // what each group's accumulator counts for, divided by the sum
-        if constexpr (G > 1) {
-            exchange[g * kQ + row] = make_float2(m, l);
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * C::kSoftmaxWarps) : "memory");
-            float2 ml[G];
-            float top = -INFINITY;  // of all groups
+            if (lane == 0) mbar_arrive(p_full + 8 * sb.slot);
+            ob = sb;
+            sb.next();
+        };
+        for (int j = 0; live && j < n; ++j) {
+            const uint32_t ts = t0 + 64 * sb.slot;
+            ok = wait(s_full + 8 * sb.slot, sb.parity);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[2][32];
+            tmem_ld32(ts, s[0]);
+            tmem_ld32(ts + 32, s[1]);
+            tmem_wait_ld();
+            tmem_settle(s[0]);
+            tmem_settle(s[1]);
+            const int rows = rows_of(block_of(j));
+            if (rows < kK) {
 #pragma unroll
-            for (int x = 0; x < G; ++x) {
-                ml[x] = exchange[x * kQ + row];
-                top = max3(top, ml[x].x, ml[x].x);
+                for (int x = 0; x < kK; ++x)
+                    if (x >= rows) s[x / 32][x % 32] = 0xff800000u;  // -inf
+                ok = clear_tail(j, rows);
+                if (!ok) break;
             }
-            l = 0.f;
+            // the running maximum, and a rescale of O and l where it has grown
+            float mx[4] = {m, m, m, m};
 #pragma unroll
-            for (int x = 0; x < G; ++x) {
-                a[x] = top == -INFINITY ? 1.f : exp2_hw((ml[x].x - top) * p.c);
-                l = fmaf(a[x], ml[x].y, l);
+            for (int x = 0; x < kK; x += 2)
+                mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x / 32][x % 32]), __uint_as_float(s[x / 32][x % 32 + 1]));
+            const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            // a NaN maximum always counts as grown, and stays
+            const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {
+                const float to = grown ? mt : m;
+                const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
+                if (j > 0) {
+                    ok = wait(o_done + 8 * ob.slot, ob.parity);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 8) {
+                        uint32_t o[8];
+                        tmem_ld8(t0 + C::kOCol + c0, o);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                        tmem_st8(t0 + C::kOCol + c0, o);
+                    }
+                }
+                l *= alpha;
+                m = to;
             }
-            m = top;
-        } else {
-            a[0] = 1.f;
+            // the weights, into the scores' first columns, and their sum
+            // (an infinite maximum makes its row NaN, as inf - inf does)
+            const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
+            F2 sum[2] = {both(0.f), both(0.f)};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    F2 v = fma2v(F2{__uint_as_float(s[half][2 * x]), __uint_as_float(s[half][2 * x + 1])}, both(p.c), bias);
+                    if ((x & 7) < kPolyOfEight)
+                        v = exp2_poly<kF16>(v);
+                    else
+                        v = F2{exp2_hw(v.x), exp2_hw(v.y)};
+                    sum[x & 1] = add2v(sum[x & 1], v);
+                    w[x] = pack2<kF16>(v.x, v.y);
+                }
+                tmem_st16(ts + 16 * half, w);
+            }
+            const F2 total = add2v(sum[0], sum[1]);
+            l += total.x + total.y;
+            tmem_wait_st();
+            hand_over();
         }
+        for (int j = 0; !live && j < n && ok; ++j) {
+            ok = wait(s_full + 8 * sb.slot, sb.parity);
+            const int rows = rows_of(block_of(j));
+            if (ok && rows < kK) ok = clear_tail(j, rows);
+            if (ok) hand_over();
+        }
+        // the last product (they complete in order). A wait tells two neighbouring phases of its
+        // barrier apart: with one o_done per buffer the phase before is over when s_full is seen
+        if (ok && n > 0) ok = wait(o_done + 8 * ((n - 1) % B), ((n - 1) / B) & 1);
         tc_fence_after();
         if (ok && live) {
             // nothing listed, or every score -inf (exp2_poly gives those a weight of 2^-126, not 0)
             const bool none = m == -INFINITY || l == 0.f;
             const float inv = none ? 0.f : 1.f / l;
             uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(q_row0 + row) * p.out_stride + (int64_t)h * D;
-            const uint32_t t0 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + C::kOCol;
-            // each group writes its share of the columns
-#pragma unroll
-            for (int c0 = g * (D / G); c0 < (g + 1) * (D / G); c0 += 32) {
-                float o[32];
-#pragma unroll
-                for (int y = 0; y < 32; ++y) o[y] = 0.f;
-#pragma unroll
-                for (int x = 0; x < G; ++x) {
-                    if (n <= x) break;  // that group had no block: its accumulator was never written
-                    uint32_t v[32];
-                    tmem_ld32(t0 + x * C::kGroupCols + c0, v);
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld32(t0 + C::kOCol + c0, o);
                     tmem_wait_ld();
-                    tmem_settle(v);
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) o[y] = fmaf(__uint_as_float(v[y]), a[x] * inv, o[y]);
+                    tmem_settle(o);
                 }
                 if (row < q_rows) {
                     uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
@@ -522,7 +506,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
                         uint32_t w[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            w[x] = none ? 0u : pack2<kF16>(o[8 * y + 2 * x], o[8 * y + 2 * x + 1]);
+                            w[x] = none ? 0u
+                                        : pack2<kF16>(__uint_as_float(o[8 * y + 2 * x]) * inv,
+                                                      __uint_as_float(o[8 * y + 2 * x + 1]) * inv);
                         d4[y] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
