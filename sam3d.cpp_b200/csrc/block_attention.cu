@@ -1,7 +1,9 @@
 // Block attention: out = softmax(scale q k^T) v of each query row over the
 // rows of its listed key blocks (64 rows each), or over its whole sequence.
 //
-// One CTA per (query block of 128 rows, head). The row maximum and sum run
+// One CTA per (query block of 128 rows, head); short blocks of grouped heads
+// share a tile, and where there are few tiles their lists are split over CTAs
+// and joined by a second kernel. The row maximum and sum run
 // along with the blocks (online softmax), so scores never leave the SM:
 //
 //   producer warp   TMA: the Q tile once, then the K and V tiles of the listed blocks into rings
@@ -46,13 +48,21 @@ constexpr float kSlack = 8.f;
 // rows x 148 heads, 0 / 1 / 2 / 3 of eight took 910 / 903 / 893 / 960 us
 constexpr int kPolyOfEight = 2;
 
+constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
+constexpr int kMaxChunks = 128;
+
 struct AttnParams {
     const int4* q_blocks;
     const int32_t* sel;  // [n_qb][heads][top], or nullptr
     int top, heads, per_kv;
-    float c;  // scale * log2(e)
+    int pack;   // heads of a group that share a tile: tile row r is query row r / pack, head r % pack
+    int chunk;  // list entries of a CTA (blockIdx.z counts the chunks), or 0: the whole list
+    float c;    // scale * log2(e)
     void* out;
     int64_t out_stride;
+    int64_t n_q;
+    float* part_o;   // [chunks][n_q][heads][D] unnormalised sums (chunk > 0)
+    float2* part_ml; // [chunks][n_q][heads] their row maximum and sum
     uint32_t* status;
 };
 
@@ -93,6 +103,12 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
     return ok != 0;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"((unsigned long long)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -262,9 +278,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    const int h = blockIdx.y;
+    const int h = blockIdx.y * p.pack;
     const int4 qb = p.q_blocks[blockIdx.x];
-    const int q_row0 = qb.x, q_rows = qb.y & kAttnRowsMask, k_row0 = qb.z, k_rows = qb.w;
+    const int q_row0 = qb.x, q_rows = (qb.y & kAttnRowsMask) * p.pack, k_row0 = qb.z, k_rows = qb.w;
     const int nkb = (k_rows + kK - 1) / kK;
     if (warp == 0) {
         // the listed blocks that exist, in list order
@@ -287,17 +303,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     tc_fence_after();
     pdl_trigger();
     const uint32_t tmem = *tmem_holder;
-    const int n = *n_listed;
-    auto block_of = [&](int j) { return p.sel ? list[j] : j; };
+    const int first = p.chunk * blockIdx.z;
+    const int n = p.chunk ? max(0, min(p.chunk, *n_listed - first)) : *n_listed;
+    auto block_of = [&](int j) { return p.sel ? list[first + j] : first + j; };
     auto rows_of = [&](int blk) { return min(kK, k_rows - blk * kK); };
 
     if (warp == kProdWarp) {
         // ================= TMA producer =================
         if (n > 0 && elect_one()) {
             constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
-            const int qc = h * D, kc = (h / p.per_kv) * D;
+            const int kc = (h / p.per_kv) * D;
             mbar_arrive_tx(q_full, C::kPanels * kQPanel);
-            for (int i = 0; i < C::kPanels; ++i) tma_load_2d(sQ + i * kQPanel, &qmap, qc + 64 * i, q_row0, q_full);
+            for (int i = 0; i < C::kPanels; ++i) tma_load_3d(sQ + i * kQPanel, &qmap, 64 * i, h, q_row0, q_full);
             int issued_k = 0, issued_v = 0;
             bool ok = true;
             Cursor<C::kKS> ks;
@@ -490,7 +507,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             // nothing listed, or every score -inf (exp2_poly gives those a weight of 2^-126, not 0)
             const bool none = m == -INFINITY || l == 0.f;
             const float inv = none ? 0.f : 1.f / l;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(q_row0 + row) * p.out_stride + (int64_t)h * D;
+            const int64_t q_row = q_row0 + row / p.pack;
+            const int head = h + row % p.pack;
+            const int64_t part = ((int64_t)blockIdx.z * p.n_q + q_row) * p.heads + head;
+            if (p.chunk && row < q_rows) p.part_ml[part] = make_float2(m, l);
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + q_row * p.out_stride + (int64_t)head * D;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t o[32];
@@ -499,18 +520,26 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
                     tmem_wait_ld();
                     tmem_settle(o);
                 }
-                if (row < q_rows) {
-                    uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
+                if (row >= q_rows) continue;
+                if (p.chunk) {
+                    if (n == 0) break;  // m = -inf: never read
+                    float4* d4 = reinterpret_cast<float4*>(p.part_o + part * D + c0);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        uint32_t w[4];
+                    for (int y = 0; y < 8; ++y)
+                        d4[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]),
+                                            __uint_as_float(o[4 * y + 2]), __uint_as_float(o[4 * y + 3]));
+                    continue;
+                }
+                uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            w[x] = none ? 0u
-                                        : pack2<kF16>(__uint_as_float(o[8 * y + 2 * x]) * inv,
-                                                      __uint_as_float(o[8 * y + 2 * x + 1]) * inv);
-                        d4[y] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                for (int y = 0; y < 4; ++y) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        w[x] = none ? 0u
+                                    : pack2<kF16>(__uint_as_float(o[8 * y + 2 * x]) * inv,
+                                                  __uint_as_float(o[8 * y + 2 * x + 1]) * inv);
+                    d4[y] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
@@ -521,6 +550,52 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::kTmemCols));
     }
+}
+
+// Joins the chunks of a row: sums weighed by 2^(c (m_z - max m)). One warp per
+// (query row, head) of the plan's blocks, D / 32 columns per lane; a chunk
+// without blocks has m = -inf and is not read.
+template <int D, bool kF16>
+__global__ void __launch_bounds__(256) join_chunks_kernel(const AttnParams p, int chunks, int64_t row0) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t q_row = row0 + item / p.heads;
+    const int head = (int)(item % p.heads);
+    if (q_row >= p.n_q) return;
+    const int64_t at = q_row * p.heads + head, step = p.n_q * p.heads;
+    float top = -INFINITY;
+    for (int z = lane; z < chunks; z += 32) {
+        const float m = p.part_ml[z * step + at].x;
+        top = max3(top, m, m);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, top, x);
+        top = max3(top, m, m);
+    }
+    float acc[D / 32], l = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
+    if (!(top == -INFINITY)) {
+#pragma unroll 4
+        for (int z = 0; z < chunks; ++z) {
+            const float2 ml = p.part_ml[z * step + at];
+            if (ml.x == -INFINITY) continue;
+            const float w = exp2_hw((ml.x - top) * p.c);
+            l = fmaf(w, ml.y, l);
+            const float* o = p.part_o + (z * step + at) * D + lane * (D / 32);
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(w, o[x], acc[x]);
+        }
+    }
+    const bool none = top == -INFINITY || l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + q_row * p.out_stride + (int64_t)head * D +
+                                                lane * (D / 32));
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) dst[x] = none ? 0u : pack2<kF16>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
 }
 
 // [rows][cols] 16-bit rows, tiles of box_rows x 64 columns with the 128-byte swizzle
@@ -541,14 +616,36 @@ s3d_status encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t
     return S3D_OK;
 }
 
+// q as [rows][heads][d]: tiles of `pack` heads x kQ / pack rows x 64 columns
+s3d_status encode_q(CUtensorMap* map, const void* base, int64_t rows, int heads, int d, int64_t stride, int pack,
+                    bool f16, char* error, uint64_t error_capacity) {
+    auto encode = get_encode_fn();
+    if (!encode) return fail(error, error_capacity, S3D_INTERNAL_ERROR, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)pack, (cuuint32_t)(kQ / pack)};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult cr = encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                               const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS)
+        return fail(error, error_capacity, S3D_INTERNAL_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    return S3D_OK;
+}
+
 template <int D, bool kF16>
 cudaError_t launch(s3dsp_context* ctx, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                   const AttnParams& p) {
+                   const AttnParams& p, int64_t row0) {
     static std::atomic<uint64_t> optin{0};
-    const cudaError_t e = smem_optin((const void*)block_attention_kernel<D, kF16>, ctx->device, optin);
+    cudaError_t e = smem_optin((const void*)block_attention_kernel<D, kF16>, ctx->device, optin);
     if (e != cudaSuccess) return e;
-    return launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
-                      ctx->stream, q, k, v, p);
+    e = launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
+                   ctx->stream, q, k, v, p);
+    if (e != cudaSuccess || !p.chunk) return e;
+    const int64_t items = (p.n_q - row0) * p.heads;
+    return launch_pdl(join_chunks_kernel<D, kF16>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, ctx->stream, p,
+                      (int)grid.z, row0);
 }
 
 }  // namespace
@@ -590,18 +687,64 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointers need 16-byte alignment");
     S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
     const bool f16 = dtype == S3DSP_F16;
+    // Heads of a group share a tile where every query block is short enough for
+    // it (without a selection, whose lists are each head's own): one pass over
+    // K and V and one tile instead of `pack`. The largest power of two that
+    // divides the group and fits.
+    const int group = heads / kv_heads;
+    int pack = 1;
+    if (!d_sel)
+        while (group % (2 * pack) == 0 && 2 * pack * plan->max_q_rows <= kQ) pack *= 2;
+    // Long lists are split where the tiles alone would leave CTA slots (two per
+    // SM) empty: chunks of equal length, at least kMinChunk blocks each, so that
+    // all lists together fill the slots once.
+    const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
+    const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
+    int chunk = 0, chunks = 1;
+    if (tiles < slots && longest > kMinChunk) {
+        const int64_t work = (d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * (heads / pack);
+        int64_t c = (work + slots - 1) / slots;
+        if (c < kMinChunk) c = kMinChunk;
+        if (c < (longest + kMaxChunks - 1) / kMaxChunks) c = (longest + kMaxChunks - 1) / kMaxChunks;
+        chunks = (int)((longest + c - 1) / c);
+        if (chunks > 1) chunk = (int)c;
+    }
     CUtensorMap qm, km, vm;
-    S3DSP_TRY(encode_rows(&qm, q, plan->n_q, qw, q_stride, kQ, f16, error, error_capacity));
+    S3DSP_TRY(encode_q(&qm, q, plan->n_q, heads, d, q_stride, pack, f16, error, error_capacity));
     // a plan without key rows lists nothing: its maps are never read through
     const bool keys = plan->n_k > 0;
     S3DSP_TRY(encode_rows(&km, keys ? k : q, keys ? plan->n_k : 1, kw, k_stride, kK, f16, error, error_capacity));
     S3DSP_TRY(encode_rows(&vm, keys ? v : q, keys ? plan->n_k : 1, kw, v_stride, kK, f16, error, error_capacity));
-    AttnParams p = {plan->q_blocks, d_sel, top, heads, heads / kv_heads, scale * 1.4426950408889634f,
-                    out, out_stride, ctx->d_status};
-    const dim3 grid((unsigned)plan->n_qb, (unsigned)heads);
-    const cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p) : launch<64, false>(ctx, grid, qm, km, vm, p))
-                                  : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p)
-                                         : launch<128, false>(ctx, grid, qm, km, vm, p));
-    if (e != cudaSuccess) return cuda_fail(error, error_capacity, e, "block_attention_kernel");
+    AttnParams p = {};
+    p.q_blocks = plan->q_blocks;
+    p.sel = d_sel;
+    p.top = top;
+    p.heads = heads;
+    p.per_kv = group;
+    p.pack = pack;
+    p.chunk = chunk;
+    p.c = scale * 1.4426950408889634f;
+    p.out = out;
+    p.out_stride = out_stride;
+    p.n_q = plan->n_q;
+    p.status = ctx->d_status;
+    char* parts = nullptr;
+    if (chunk) {
+        const size_t rows = (size_t)chunks * plan->n_q * heads;
+        S3DSP_CUDA(malloc_async(&parts, rows * (d * sizeof(float) + sizeof(float2)), ctx->stream), "chunk sums");
+        p.part_o = reinterpret_cast<float*>(parts);
+        p.part_ml = reinterpret_cast<float2*>(parts + rows * d * sizeof(float));
+    }
+    const dim3 grid((unsigned)plan->n_qb, (unsigned)(heads / pack), (unsigned)chunks);
+    const int64_t row0 = plan->first_q;
+    cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p, row0)
+                                   : launch<64, false>(ctx, grid, qm, km, vm, p, row0))
+                            : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p, row0)
+                                   : launch<128, false>(ctx, grid, qm, km, vm, p, row0));
+    if (parts) {
+        const cudaError_t f = cudaFreeAsync(parts, ctx->stream);
+        if (e == cudaSuccess) e = f;
+    }
+    if (e != cudaSuccess) return cuda_fail(error, error_capacity, e, "block_attention kernels");
     return S3D_OK;
 }

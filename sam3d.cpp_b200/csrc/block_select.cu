@@ -256,8 +256,8 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     const int64_t fit = max_kb > 0 ? (kSmemOptIn / 8 - 256 * kAttnGroupRows) / max_kb : kAttnGroupRows;
     const int group = fit >= kAttnGroupRows ? kAttnGroupRows : fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 1;
     auto* plan = new (std::nothrow) s3dsp_attn_plan();
-    // one upload: q_blocks int4, k_blocks int2, groups int2, pairs int2, first_kb int
-    const size_t bytes = (size_t)nqb * (sizeof(int4) + 2 * sizeof(int2) + sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
+    // one upload: q_blocks int4, k_blocks int2, groups int2, first_kb int
+    const size_t bytes = (size_t)nqb * (sizeof(int4) + sizeof(int2) + sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
     char* host = plan ? static_cast<char*>(::operator new(bytes, std::nothrow)) : nullptr;
     if (!host) {
         delete plan;
@@ -266,16 +266,16 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     int4* qb = reinterpret_cast<int4*>(host);
     int2* kb = reinterpret_cast<int2*>(qb + nqb);
     int2* groups = kb + nkb;
-    int2* pairs = groups + nqb;
-    int* first_kb = reinterpret_cast<int*>(pairs + nqb);
-    int64_t iq = 0, ik = 0, ig = 0, ip = 0;
+    int* first_kb = reinterpret_cast<int*>(groups + nqb);
+    int64_t iq = 0, ik = 0, ig = 0;
     for (int64_t s = 0; s < n_seq; ++s) {
         const int64_t q0 = h_q_offsets[s], ql = h_q_offsets[s + 1] - q0, k0 = ko[s], kl = ko[s + 1] - k0;
         const int64_t nb = ceil_div(ql, kAttnQRows);
         for (int64_t b = 0; b < nb; ++b) {
             const int64_t left = ql - b * kAttnQRows;
             if (b % group == 0) groups[ig++] = make_int2((int)iq, (int)(nb - b < group ? nb - b : group));
-            if (b % 2 == 0) pairs[ip++] = make_int2((int)iq, nb - b < 2 ? 1 : 2);
+            plan->sum_kb += ceil_div(kl, kAttnKRows);
+            if (plan->max_q_rows < left) plan->max_q_rows = (int)(left < kAttnQRows ? left : kAttnQRows);
             first_kb[iq] = (int)ik;
             qb[iq++] = make_int4((int)(q0 + b * kAttnQRows),
                                  (int)((left < kAttnQRows ? left : kAttnQRows) | (b << kAttnRowsBits)), (int)k0, (int)kl);
@@ -288,8 +288,8 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     plan->device = ctx->device;
     plan->self = self;
     plan->n_q = nq, plan->n_k = nk;
-    plan->n_seq = n_seq;
-    plan->n_qb = (int)nqb, plan->n_kb = (int)nkb, plan->n_groups = (int)ig, plan->n_pairs = (int)ip;
+    plan->first_q = h_q_offsets[0];
+    plan->n_qb = (int)nqb, plan->n_kb = (int)nkb, plan->n_groups = (int)ig;
     plan->max_kb = (int)max_kb;
     plan->group = group;
     cudaError_t e = malloc_async(&plan->mem, bytes, ctx->stream);
@@ -306,8 +306,7 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     plan->q_blocks = static_cast<int4*>(plan->mem);
     plan->k_blocks = reinterpret_cast<int2*>(plan->q_blocks + nqb);
     plan->groups = plan->k_blocks + nkb;
-    plan->pairs = plan->groups + nqb;
-    plan->first_kb = reinterpret_cast<int*>(plan->pairs + nqb);
+    plan->first_kb = reinterpret_cast<int*>(plan->groups + nqb);
     *out = plan;
     return S3D_OK;
 }

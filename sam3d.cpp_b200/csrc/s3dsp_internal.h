@@ -84,15 +84,16 @@ struct s3dsp_attn_plan {
     int device = 0;
     bool self = false;               // the key rows are the query rows
     int64_t n_q = 0, n_k = 0;        // rows the plan spans (the last offsets)
-    int64_t n_seq = 0;
-    int n_qb = 0, n_kb = 0, n_groups = 0, n_pairs = 0;
+    int64_t first_q = 0;             // first query row of the first sequence
+    int64_t sum_kb = 0;              // over the query blocks: their sequence's key blocks
+    int max_q_rows = 0;              // most rows of a query block
+    int n_qb = 0, n_kb = 0, n_groups = 0;
     int max_kb = 0;                  // most key blocks of a sequence
     int group = 1;                   // query blocks of a selection group
     void* mem = nullptr;
     int4* q_blocks = nullptr;        // [n_qb] {first row, rows | index in the sequence << 8, first key row, key rows}
     int2* k_blocks = nullptr;        // [n_kb] {first row, rows}
     int2* groups = nullptr;          // [n_groups] {first query block, up to `group` blocks of one sequence}
-    int2* pairs = nullptr;           // [n_pairs] {first query block, 1 or 2 blocks of one sequence}
     int* first_kb = nullptr;         // [n_qb] first key block of the block's sequence
 };
 
