@@ -50,19 +50,21 @@ constexpr int kPolyOfEight = 2;
 
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
+constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
 
 struct AttnParams {
     const int4* q_blocks;
     const int32_t* sel;  // [n_qb][heads][top], or nullptr
     int top, heads, per_kv;
     int pack;   // heads of a group that share a tile: tile row r is query row r / pack, head r % pack
-    int chunk;  // list entries of a CTA (blockIdx.z counts the chunks), or 0: the whole list
+    int n_qb;   // tile t: query block t % n_qb, heads from (t / n_qb) * pack
+    int chunk, chunks;  // CTAs that share a tile's list, and list entries of each
     float c;    // scale * log2(e)
     void* out;
     int64_t out_stride;
-    int64_t n_q;
-    float* part_o;   // [chunks][n_q][heads][D] unnormalised sums (chunk > 0)
-    float2* part_ml; // [chunks][n_q][heads] their row maximum and sum
+    int tile_rows;   // most rows of a tile
+    float* part_o;   // [tiles][chunks][tile_rows][D] unnormalised sums
+    float2* part_ml; // [tiles][chunks][tile_rows] their row maximum and sum
     uint32_t* status;
 };
 
@@ -278,15 +280,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    const int h = blockIdx.y * p.pack;
-    const int4 qb = p.q_blocks[blockIdx.x];
+    const bool split = p.chunks > 1;
+    const int tile = split ? (int)blockIdx.x / p.chunks : (int)blockIdx.x;
+    const int first = split ? (int)blockIdx.x % p.chunks * p.chunk : 0;
+    const int bq = tile % p.n_qb, h = tile / p.n_qb * p.pack;
+    const int4 qb = p.q_blocks[bq];
     const int q_row0 = qb.x, q_rows = (qb.y & kAttnRowsMask) * p.pack, k_row0 = qb.z, k_rows = qb.w;
     const int nkb = (k_rows + kK - 1) / kK;
     if (warp == 0) {
         // the listed blocks that exist, in list order
         int n = nkb;
         if (p.sel) {
-            const int32_t* row = p.sel + ((int64_t)blockIdx.x * p.heads + h) * p.top;
+            const int32_t* row = p.sel + ((int64_t)bq * p.heads + h) * p.top;
             n = 0;
             for (int i0 = 0; i0 < p.top; i0 += 32) {
                 const int e = i0 + lane < p.top ? __ldg(row + i0 + lane) : -1;
@@ -303,8 +308,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     tc_fence_after();
     pdl_trigger();
     const uint32_t tmem = *tmem_holder;
-    const int first = p.chunk * blockIdx.z;
-    const int n = p.chunk ? max(0, min(p.chunk, *n_listed - first)) : *n_listed;
+    const int n = split ? max(0, min(p.chunk, *n_listed - first)) : *n_listed;
     auto block_of = [&](int j) { return p.sel ? list[first + j] : first + j; };
     auto rows_of = [&](int blk) { return min(kK, k_rows - blk * kK); };
 
@@ -509,8 +513,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             const float inv = none ? 0.f : 1.f / l;
             const int64_t q_row = q_row0 + row / p.pack;
             const int head = h + row % p.pack;
-            const int64_t part = ((int64_t)blockIdx.z * p.n_q + q_row) * p.heads + head;
-            if (p.chunk && row < q_rows) p.part_ml[part] = make_float2(m, l);
+            const int64_t part = (int64_t)blockIdx.x * p.tile_rows + row;
+            if (split && row < q_rows) p.part_ml[part] = make_float2(m, l);
             uint16_t* dst = static_cast<uint16_t*>(p.out) + q_row * p.out_stride + (int64_t)head * D;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -521,7 +525,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
                     tmem_settle(o);
                 }
                 if (row >= q_rows) continue;
-                if (p.chunk) {
+                if (split) {
                     if (n == 0) break;  // m = -inf: never read
                     float4* d4 = reinterpret_cast<float4*>(p.part_o + part * D + c0);
 #pragma unroll
@@ -552,21 +556,24 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     }
 }
 
-// Joins the chunks of a row: sums weighed by 2^(c (m_z - max m)). One warp per
-// (query row, head) of the plan's blocks, D / 32 columns per lane; a chunk
-// without blocks has m = -inf and is not read.
+// Joins the chunks of a tile's rows: sums weighed by 2^(c (m_z - max m)).
+// One warp per row, D / 32 columns per lane; a chunk without blocks has
+// m = -inf and is not read.
 template <int D, bool kF16>
-__global__ void __launch_bounds__(256) join_chunks_kernel(const AttnParams p, int chunks, int64_t row0) {
+__global__ void __launch_bounds__(256) join_chunks_kernel(const AttnParams p, int64_t items) {
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t q_row = row0 + item / p.heads;
-    const int head = (int)(item % p.heads);
-    if (q_row >= p.n_q) return;
-    const int64_t at = q_row * p.heads + head, step = p.n_q * p.heads;
+    if (item >= items) return;
+    const int tile = (int)(item / p.tile_rows), row = (int)(item % p.tile_rows);
+    const int4 qb = p.q_blocks[tile % p.n_qb];
+    if (row >= (qb.y & kAttnRowsMask) * p.pack) return;
+    const int64_t q_row = qb.x + row / p.pack, step = p.tile_rows;
+    const int64_t at = (int64_t)tile * p.chunks * step + row;
+    const int head = tile / p.n_qb * p.pack + row % p.pack;
     float top = -INFINITY;
-    for (int z = lane; z < chunks; z += 32) {
+    for (int z = lane; z < p.chunks; z += 32) {
         const float m = p.part_ml[z * step + at].x;
         top = max3(top, m, m);
     }
@@ -580,7 +587,7 @@ __global__ void __launch_bounds__(256) join_chunks_kernel(const AttnParams p, in
     for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
     if (!(top == -INFINITY)) {
 #pragma unroll 4
-        for (int z = 0; z < chunks; ++z) {
+        for (int z = 0; z < p.chunks; ++z) {
             const float2 ml = p.part_ml[z * step + at];
             if (ml.x == -INFINITY) continue;
             const float w = exp2_hw((ml.x - top) * p.c);
@@ -636,16 +643,15 @@ s3d_status encode_q(CUtensorMap* map, const void* base, int64_t rows, int heads,
 
 template <int D, bool kF16>
 cudaError_t launch(s3dsp_context* ctx, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
-                   const AttnParams& p, int64_t row0) {
+                   const AttnParams& p) {
     static std::atomic<uint64_t> optin{0};
     cudaError_t e = smem_optin((const void*)block_attention_kernel<D, kF16>, ctx->device, optin);
     if (e != cudaSuccess) return e;
     e = launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
                    ctx->stream, q, k, v, p);
-    if (e != cudaSuccess || !p.chunk) return e;
-    const int64_t items = (p.n_q - row0) * p.heads;
-    return launch_pdl(join_chunks_kernel<D, kF16>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, ctx->stream, p,
-                      (int)grid.z, row0);
+    if (e != cudaSuccess || p.chunks == 1) return e;
+    const int64_t items = (int64_t)grid.x / p.chunks * p.tile_rows;
+    return launch_pdl(join_chunks_kernel<D, kF16>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, ctx->stream, p, items);
 }
 
 }  // namespace
@@ -695,19 +701,24 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     int pack = 1;
     if (!d_sel)
         while (group % (2 * pack) == 0 && 2 * pack * plan->max_q_rows <= kQ) pack *= 2;
-    // Long lists are split where the tiles alone would leave CTA slots (two per
-    // SM) empty: chunks of equal length, at least kMinChunk blocks each, so that
-    // all lists together fill the slots once.
+    // Where the tiles leave half or more of the CTA slots (two per SM) empty,
+    // several CTAs share a tile's list: chunks of equal length, by what the
+    // lists hold together, so that they fill the slots about once however the
+    // lengths differ. A chunk has at least kMinChunk blocks, and the split has
+    // to save kMinSaved: a block takes a CTA about 0.9 us, the joining kernel
+    // and its traffic about 8. (8 rows over 92k keys, 4 key heads: 527 us
+    // without, 68 with. Sharing only the tiles of a last, half empty wave was
+    // measured too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on
+    // an SM runs 1.2x as fast as one of two.)
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
+    if (tiles > 0x3fffffff) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "too many query blocks times heads");
     const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
-    int chunk = 0, chunks = 1;
-    if (tiles < slots && longest > kMinChunk) {
-        const int64_t work = (d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * (heads / pack);
-        int64_t c = (work + slots - 1) / slots;
-        if (c < kMinChunk) c = kMinChunk;
-        if (c < (longest + kMaxChunks - 1) / kMaxChunks) c = (longest + kMaxChunks - 1) / kMaxChunks;
-        chunks = (int)((longest + c - 1) / c);
-        if (chunks > 1) chunk = (int)c;
+    int64_t chunk = longest, chunks = 1;
+    if (tiles <= slots / 2) {
+        chunk = ((d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * (heads / pack) + slots - 1) / slots;
+        if (chunk < kMinChunk) chunk = kMinChunk;
+        if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
+        if (longest - chunk >= kMinSaved) chunks = (longest + chunk - 1) / chunk;
     }
     CUtensorMap qm, km, vm;
     S3DSP_TRY(encode_q(&qm, q, plan->n_q, heads, d, q_stride, pack, f16, error, error_capacity));
@@ -722,25 +733,25 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.heads = heads;
     p.per_kv = group;
     p.pack = pack;
-    p.chunk = chunk;
+    p.n_qb = plan->n_qb;
+    p.chunk = (int)chunk;
+    p.chunks = (int)chunks;
+    p.tile_rows = plan->max_q_rows * pack;
     p.c = scale * 1.4426950408889634f;
     p.out = out;
     p.out_stride = out_stride;
-    p.n_q = plan->n_q;
     p.status = ctx->d_status;
     char* parts = nullptr;
-    if (chunk) {
-        const size_t rows = (size_t)chunks * plan->n_q * heads;
+    if (chunks > 1) {
+        const size_t rows = (size_t)tiles * chunks * p.tile_rows;
         S3DSP_CUDA(malloc_async(&parts, rows * (d * sizeof(float) + sizeof(float2)), ctx->stream), "chunk sums");
         p.part_o = reinterpret_cast<float*>(parts);
         p.part_ml = reinterpret_cast<float2*>(parts + rows * d * sizeof(float));
     }
-    const dim3 grid((unsigned)plan->n_qb, (unsigned)(heads / pack), (unsigned)chunks);
-    const int64_t row0 = plan->first_q;
-    cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p, row0)
-                                   : launch<64, false>(ctx, grid, qm, km, vm, p, row0))
-                            : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p, row0)
-                                   : launch<128, false>(ctx, grid, qm, km, vm, p, row0));
+    const dim3 grid((unsigned)(tiles * chunks));
+    cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p) : launch<64, false>(ctx, grid, qm, km, vm, p))
+                            : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p)
+                                   : launch<128, false>(ctx, grid, qm, km, vm, p));
     if (parts) {
         const cudaError_t f = cudaFreeAsync(parts, ctx->stream);
         if (e == cudaSuccess) e = f;

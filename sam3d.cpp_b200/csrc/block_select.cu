@@ -12,9 +12,13 @@
 //
 //   block_mean_kernel   one pass over q and k (memory bound): a warp lane owns eight columns, eight
 //                       warps share the block's rows, f64 sums joined in warp order
-//   block_score_kernel  one CTA per (up to kGroup query blocks of a sequence, head): scores into shared
-//                       memory, then one warp per row finds the top-th largest key by bisection over
-//                       the ordered bits and writes the chosen indices in ascending order
+//   block_score_kernel  scores of 32 query blocks x 64 key blocks of one sequence and head, a tile
+//                       product in f64 (the f64 pipe bounds it: 64 FMAs a cycle and SM), written as
+//                       64-bit keys whose unsigned order is the scores'
+//   top_warp_kernel     one warp per (query block, head): the top-th largest key by bisection, the
+//                       keys' upper halves in registers; the chosen indices in ascending order
+//   top_block_kernel    the same with one CTA per row and the keys in shared memory, for sequences
+//                       of more key blocks than a warp's registers take
 #include "s3dsp_internal.h"
 
 using namespace s3dsp;
@@ -23,8 +27,11 @@ namespace {
 
 constexpr int kMeanThreads = 256;
 constexpr int kMeanCols = 256;  // columns per CTA of the mean kernel: 32 lanes x 8
-constexpr int kScoreThreads = 256;
-constexpr int kGroup = kAttnGroupRows;  // most query blocks per CTA of the score kernel
+constexpr int kScoreThreads = 128;
+constexpr int kTileQ = kAttnGroupRows, kTileK = 64, kTileD = 32;  // of the score kernel
+constexpr int kWarpKeys = 32;                                     // key blocks per lane of top_warp_kernel
+constexpr int kMaxKeys = 28000;                                   // key blocks of a sequence: top_block_kernel's memory
+constexpr size_t kScoreBytes = (size_t)1 << 29;                   // scratch of scores that a pass over heads may take
 
 template <typename T>
 __device__ __forceinline__ double to_d(T v);
@@ -49,8 +56,8 @@ struct MeanParams {
     int n_qb, n_kb;
     const int4* q_blocks;
     const int2* k_blocks;
-    double* q_mean;   // [n_qb][qw]
-    double* k_mean;   // [kw][n_kb]: a score CTA's threads read neighbouring blocks
+    double* q_mean;  // [n_qb][qw]
+    double* k_mean;  // [n_kb][kw]
 };
 
 template <typename T, bool kVec>
@@ -106,10 +113,7 @@ __global__ void __launch_bounds__(kMeanThreads) block_mean_kernel(MeanParams p) 
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += part[w][threadIdx.x];
     s /= rows;
-    if (is_k)
-        p.k_mean[(int64_t)col * p.n_kb + b] = s;
-    else
-        p.q_mean[(int64_t)b * p.qw + col] = s;
+    (is_k ? p.k_mean + (int64_t)b * p.kw : p.q_mean + (int64_t)b * p.qw)[col] = s;
 }
 
 struct ScoreParams {
@@ -118,9 +122,11 @@ struct ScoreParams {
     const int* first_kb;    // [n_qb] first key block of the block's sequence
     const double* q_mean;
     const double* k_mean;
-    int qw, n_kb, d, heads, per_kv, top, keep_local;
-    int max_kb;             // row length of the score table
-    int32_t* sel;           // [n_qb][heads][top]
+    int qw, kw, n_qb, d, heads, per_kv, top, keep_local;
+    int head0, head_count;  // heads of this pass
+    int max_kb;             // keys of a row
+    unsigned long long* keys;  // [n_qb][head_count][max_kb]
+    int32_t* sel;              // [n_qb][heads][top]
 };
 
 // f64 -> u64 whose unsigned order is the scores' order; NaN lowest
@@ -130,85 +136,205 @@ __device__ __forceinline__ unsigned long long ordered(double v) {
     return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-__global__ void __launch_bounds__(kScoreThreads) block_score_kernel(ScoreParams p) {
-    extern __shared__ double sm[];
-    double* qm = sm;                                  // [d][kGroup]
-    double* score = sm + (size_t)p.d * kGroup;        // [count][max_kb] as ordered keys
+// A thread owns 4 query blocks x 4 key blocks; every score is summed over the
+// head's columns in order, so that equal blocks have equal scores.
+__global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreParams p) {
+    __shared__ __align__(16) double qs[kTileD][kTileQ + 2], ks[kTileD][kTileK + 2];
     pdl_wait();
     pdl_trigger();
     const int2 grp = p.groups[blockIdx.x];
-    const int h = blockIdx.y;
-    const int b0 = grp.x, count = grp.y;
+    const int b0 = grp.x, count = grp.y, c0 = blockIdx.y * kTileK, h = p.head0 + blockIdx.z;
     const int4 qb0 = p.q_blocks[b0];
     const int nkb = (qb0.w + kAttnKRows - 1) / kAttnKRows;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (nkb > p.top) {
-        for (int e = threadIdx.x; e < p.d * kGroup; e += kScoreThreads) {
-            const int r = e / p.d, j = e - r * p.d;
-            qm[j * kGroup + r] = r < count ? p.q_mean[(int64_t)(b0 + r) * p.qw + h * p.d + j] : 0.0;
-        }
+    if (c0 >= nkb || nkb <= p.top) return;  // all blocks are taken: no scores needed
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const double* qm = p.q_mean + (int64_t)b0 * p.qw + (int64_t)h * p.d;
+    const double* km = p.k_mean + (int64_t)(p.first_kb[b0] + c0) * p.kw + (int64_t)(h / p.per_kv) * p.d;
+    double acc[4][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = 0.0;
+    for (int j0 = 0; j0 < p.d; j0 += kTileD) {
+        const int dn = min(kTileD, p.d - j0);
+        const int j = threadIdx.x & (kTileD - 1);
+#pragma unroll
+        for (int r = threadIdx.x / kTileD; r < kTileQ; r += kScoreThreads / kTileD)
+            qs[j][r] = r < count && j < dn ? qm[(int64_t)r * p.qw + j0 + j] : 0.0;
+#pragma unroll
+        for (int c = threadIdx.x / kTileD; c < kTileK; c += kScoreThreads / kTileD)
+            ks[j][c] = c0 + c < nkb && j < dn ? km[(int64_t)c * p.kw + j0 + j] : 0.0;
         __syncthreads();
-        const double* km = p.k_mean + (int64_t)(h / p.per_kv) * p.d * p.n_kb + p.first_kb[b0];
-        for (int c = threadIdx.x; c < nkb; c += kScoreThreads) {
-            double acc[kGroup];
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) acc[r] = 0.0;
 #pragma unroll 4
-            for (int j = 0; j < p.d; ++j) {
-                const double kv = km[(int64_t)j * p.n_kb + c];
+        for (int i = 0; i < dn; ++i) {
+            const double2 q01 = *reinterpret_cast<const double2*>(&qs[i][4 * ty]);
+            const double2 q23 = *reinterpret_cast<const double2*>(&qs[i][4 * ty + 2]);
+            const double2 k01 = *reinterpret_cast<const double2*>(&ks[i][2 * tx]);
+            const double2 k23 = *reinterpret_cast<const double2*>(&ks[i][2 * tx + 32]);
+            const double qv[4] = {q01.x, q01.y, q23.x, q23.y}, kv[4] = {k01.x, k01.y, k23.x, k23.y};
 #pragma unroll
-                for (int r = 0; r < kGroup; ++r) acc[r] = fma(qm[j * kGroup + r], kv, acc[r]);
-            }
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int r = 0; r < kGroup; ++r)
-                if (r < count) {
-                    unsigned long long key = ordered(acc[r]);
-                    if (p.keep_local) {
-                        // the key blocks of the query block's own rows come first
-                        const int own = ((qb0.y >> kAttnRowsBits) + r) * (kAttnQRows / kAttnKRows);
-                        if (c >= own && c < own + kAttnQRows / kAttnKRows) key = ~0ull;
-                    }
-                    reinterpret_cast<unsigned long long*>(score)[(size_t)r * p.max_kb + c] = key;
-                }
+                for (int y = 0; y < 4; ++y) acc[x][y] = fma(qv[x], kv[y], acc[x][y]);
         }
         __syncthreads();
     }
-    for (int r = warp; r < count; r += kScoreThreads / 32) {
-        int32_t* out = p.sel + ((int64_t)(b0 + r) * p.heads + h) * p.top;
-        if (nkb <= p.top) {  // all of them
-            for (int i = lane; i < p.top; i += 32) out[i] = i < nkb ? i : -1;
-            continue;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const int r = 4 * ty + x;
+        if (r >= count) break;
+        // the key blocks of the query block's own rows come first
+        const int own = p.keep_local ? ((qb0.y >> kAttnRowsBits) + r) * (kAttnQRows / kAttnKRows) : -2;
+        unsigned long long* row = p.keys + ((int64_t)(b0 + r) * p.head_count + blockIdx.z) * p.max_kb;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int c = c0 + 2 * tx + (y & 1) + 32 * (y >> 1);
+            if (c < nkb) row[c] = c >= own && c < own + kAttnQRows / kAttnKRows ? ~0ull : ordered(acc[x][y]);
         }
-        const unsigned long long* key = reinterpret_cast<unsigned long long*>(score) + (size_t)r * p.max_kb;
-        // the largest t with at least `top` keys >= t, bit by bit from the top
-        unsigned long long t = 0ull;
-        for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long cand = t | (1ull << bit);
-            int m = 0;
-            for (int c = lane; c < nkb; c += 32) m += key[c] >= cand;
-            m = __reduce_add_sync(0xffffffffu, m);
-            if (m >= p.top) {
-                t = cand;
-                if (m == p.top) break;
+    }
+}
+
+// Writes the lane's index c to the row's list when it is taken: keys above the
+// threshold, and the first `ties` of those equal to it. A warp's step of 32.
+__device__ __forceinline__ void emit(int32_t* out, int c, bool above, bool equal, int lane, int& done, int& ties) {
+    const unsigned below = (1u << lane) - 1u, em = __ballot_sync(0xffffffffu, equal);
+    const bool take = above || (equal && __popc(em & below) < ties);
+    const unsigned tm = __ballot_sync(0xffffffffu, take);
+    if (take) out[done + __popc(tm & below)] = c;
+    done += __popc(tm);
+    ties -= min(ties, __popc(em));
+}
+
+__global__ void __launch_bounds__(128) top_warp_kernel(const ScoreParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (item >= (int64_t)p.n_qb * p.head_count) return;
+    const int b = (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
+    const int nkb = (p.q_blocks[b].w + kAttnKRows - 1) / kAttnKRows;
+    int32_t* out = p.sel + ((int64_t)b * p.heads + h) * p.top;
+    if (nkb <= p.top) {  // all of them
+        for (int i = lane; i < p.top; i += 32) out[i] = i < nkb ? i : -1;
+        return;
+    }
+    const uint2* key = reinterpret_cast<const uint2*>(p.keys + item * p.max_kb);  // {lower, upper half}
+    const int steps = (nkb + 31) / 32;
+    uint32_t hi[kWarpKeys];
+    uint32_t lo_bound = 0xffffffffu, hi_bound = 0u;
+#pragma unroll
+    for (int i = 0; i < kWarpKeys; ++i) {
+        const int c = 32 * i + lane;
+        hi[i] = 0u;
+        if (i < steps && c < nkb) {
+            hi[i] = key[c].y;
+            lo_bound = min(lo_bound, hi[i]);
+            hi_bound = max(hi_bound, hi[i]);
+        }
+    }
+    // the largest t with at least `top` upper halves >= t: count(lo) >= top > count(up)
+    uint32_t lo = __reduce_min_sync(0xffffffffu, lo_bound);
+    uint64_t up = (uint64_t)__reduce_max_sync(0xffffffffu, hi_bound) + 1;
+    int at_lo = nkb;
+    while (up - lo > 1 && at_lo != p.top) {
+        const uint32_t mid = (uint32_t)(lo + (up - lo) / 2);
+        int m = 0;
+#pragma unroll
+        for (int i = 0; i < kWarpKeys; ++i)
+            if (i < steps) m += hi[i] >= mid;  // the padding's 0 is below every mid > lo >= 0
+        m = __reduce_add_sync(0xffffffffu, m);
+        if (m >= p.top)
+            lo = mid, at_lo = m;
+        else
+            up = mid;
+    }
+    int done = 0, ties = 0;
+    if (at_lo == p.top) {  // those >= lo are the list
+#pragma unroll
+        for (int i = 0; i < kWarpKeys; ++i)
+            if (i < steps) emit(out, 32 * i + lane, 32 * i + lane < nkb && hi[i] >= lo, false, lane, done, ties);
+        return;
+    }
+    // several keys share the threshold's upper half: bisect their lower halves
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < kWarpKeys; ++i)
+        if (i < steps) above += 32 * i + lane < nkb && hi[i] > lo;
+    above = __reduce_add_sync(0xffffffffu, above);
+    const int want = p.top - above;
+    uint32_t t = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = t | (1u << bit);
+        int m = 0;
+        for (int i = 0; i < steps; ++i) {
+            const int c = 32 * i + lane;
+            if (c < nkb) {
+                const uint2 k = key[c];
+                m += k.y == lo && k.x >= cand;
             }
         }
-        int above = 0;
-        for (int c = lane; c < nkb; c += 32) above += key[c] > t;
-        above = __reduce_add_sync(0xffffffffu, above);
-        // every key above t, and the first of those equal to it, in index order;
-        // when exactly `top` keys are >= t the equal ones all fit
-        int ties = p.top - above, done = 0;
-        for (int c0 = 0; c0 < nkb && done < p.top; c0 += 32) {
-            const int c = c0 + lane;
-            const unsigned long long kc = c < nkb ? key[c] : 0ull;
-            const bool gt = c < nkb && kc > t, eq = c < nkb && kc == t;
-            const unsigned em = __ballot_sync(0xffffffffu, eq), lt = (1u << lane) - 1u;
-            const bool take = gt || (eq && __popc(em & lt) < ties);
-            const unsigned tm = __ballot_sync(0xffffffffu, take);
-            if (take) out[done + __popc(tm & lt)] = c;
-            done += __popc(tm);
-            ties -= min(ties, __popc(em));
+        if (__reduce_add_sync(0xffffffffu, m) >= want) t = cand;
+    }
+    int over = 0;
+    for (int i = 0; i < steps; ++i) {
+        const int c = 32 * i + lane;
+        if (c < nkb) {
+            const uint2 k = key[c];
+            over += k.y == lo && k.x > t;
         }
+    }
+    ties = want - __reduce_add_sync(0xffffffffu, over);
+    for (int i = 0; i < steps; ++i) {
+        const int c = 32 * i + lane;
+        const uint2 k = c < nkb ? key[c] : make_uint2(0u, 0u);
+        emit(out, c, c < nkb && (k.y > lo || (k.y == lo && k.x > t)), c < nkb && k.y == lo && k.x == t, lane, done, ties);
+    }
+}
+
+constexpr int kTopThreads = 512;
+__global__ void __launch_bounds__(kTopThreads) top_block_kernel(const ScoreParams p) {
+    extern __shared__ unsigned long long key[];  // [max_kb], then two counters
+    int* total = reinterpret_cast<int*>(key + p.max_kb);
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int64_t item = blockIdx.x;
+    const int b = (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
+    const int nkb = (p.q_blocks[b].w + kAttnKRows - 1) / kAttnKRows;
+    int32_t* out = p.sel + ((int64_t)b * p.heads + h) * p.top;
+    if (nkb <= p.top) {
+        for (int i = threadIdx.x; i < p.top; i += kTopThreads) out[i] = i < nkb ? i : -1;
+        return;
+    }
+    for (int c = threadIdx.x; c < nkb; c += kTopThreads) key[c] = p.keys[item * p.max_kb + c];
+    if (threadIdx.x < 2) total[threadIdx.x] = 0;
+    __syncthreads();
+    int turn = 0;  // the counter in use; the other one is cleared meanwhile
+    auto count = [&](unsigned long long t) {
+        int m = 0;
+        for (int c = threadIdx.x; c < nkb; c += kTopThreads) m += key[c] >= t;
+        m = __reduce_add_sync(0xffffffffu, m);
+        if (lane == 0) atomicAdd(&total[turn], m);
+        __syncthreads();
+        m = total[turn];
+        if (threadIdx.x == 0) total[turn ^ 1] = 0;
+        turn ^= 1;
+        __syncthreads();
+        return m;
+    };
+    unsigned long long t = 0ull;
+    for (int bit = 63; bit >= 0; --bit) {
+        const unsigned long long cand = t | (1ull << bit);
+        const int m = count(cand);
+        if (m >= p.top) t = cand;
+        if (m == p.top) break;
+    }
+    int ties = p.top - (t == ~0ull ? 0 : count(t + 1)), done = 0;
+    if (threadIdx.x >= 32) return;
+    for (int c0 = 0; c0 < nkb && done < p.top; c0 += 32) {
+        const int c = c0 + lane;
+        const unsigned long long k = c < nkb ? key[c] : 0ull;
+        emit(out, c, c < nkb && k > t, c < nkb && k == t, lane, done, ties);
     }
 }
 
@@ -251,10 +377,6 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
         const int64_t m = ceil_div(ko[s + 1] - ko[s], kAttnKRows);
         if (m > max_kb) max_kb = m;
     }
-    // query blocks of a selection group: as many score rows as fit in shared
-    // memory beside 16 mean rows of the widest head
-    const int64_t fit = max_kb > 0 ? (kSmemOptIn / 8 - 256 * kAttnGroupRows) / max_kb : kAttnGroupRows;
-    const int group = fit >= kAttnGroupRows ? kAttnGroupRows : fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 1;
     auto* plan = new (std::nothrow) s3dsp_attn_plan();
     // one upload: q_blocks int4, k_blocks int2, groups int2, first_kb int
     const size_t bytes = (size_t)nqb * (sizeof(int4) + sizeof(int2) + sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
@@ -273,7 +395,8 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
         const int64_t nb = ceil_div(ql, kAttnQRows);
         for (int64_t b = 0; b < nb; ++b) {
             const int64_t left = ql - b * kAttnQRows;
-            if (b % group == 0) groups[ig++] = make_int2((int)iq, (int)(nb - b < group ? nb - b : group));
+            if (b % kAttnGroupRows == 0)
+                groups[ig++] = make_int2((int)iq, (int)(nb - b < kAttnGroupRows ? nb - b : kAttnGroupRows));
             plan->sum_kb += ceil_div(kl, kAttnKRows);
             if (plan->max_q_rows < left) plan->max_q_rows = (int)(left < kAttnQRows ? left : kAttnQRows);
             first_kb[iq] = (int)ik;
@@ -288,10 +411,8 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     plan->device = ctx->device;
     plan->self = self;
     plan->n_q = nq, plan->n_k = nk;
-    plan->first_q = h_q_offsets[0];
     plan->n_qb = (int)nqb, plan->n_kb = (int)nkb, plan->n_groups = (int)ig;
     plan->max_kb = (int)max_kb;
-    plan->group = group;
     cudaError_t e = malloc_async(&plan->mem, bytes, ctx->stream);
     if (e == cudaSuccess) {
         // pageable memory: staged before the call returns
@@ -358,33 +479,52 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
     const size_t es = dtype_size(dtype);
     if (((uintptr_t)q | (uintptr_t)k) & (es - 1))
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointer not aligned to its type");
-    const size_t smem = sizeof(double) * ((size_t)d * kGroup + (size_t)plan->group * plan->max_kb);
-    if (smem > (size_t)kSmemOptIn)
-        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "a sequence has %d key blocks: more than a selection takes",
-                    plan->max_kb);
+    if (plan->max_kb > kMaxKeys)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "a sequence has %d key blocks (at most %d)",
+                    plan->max_kb, kMaxKeys);
     S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
     static std::atomic<uint64_t> optin{0};
-    S3DSP_CUDA(smem_optin((const void*)block_score_kernel, ctx->device, optin), "block_score_kernel");
+    S3DSP_CUDA(smem_optin((const void*)top_block_kernel, ctx->device, optin), "top_block_kernel");
     double* means = nullptr;
     const size_t n_qm = (size_t)plan->n_qb * qw, n_km = (size_t)plan->n_kb * kw;
-    S3DSP_CUDA(malloc_async(&means, (n_qm + n_km) * sizeof(double), ctx->stream), "block means");
+    // scores of as many heads at a time as kScoreBytes take (one at least)
+    const size_t row_bytes = (size_t)plan->n_qb * plan->max_kb * sizeof(unsigned long long);
+    const bool scored = plan->max_kb > top;
+    int64_t pass = scored && row_bytes * heads > kScoreBytes ? kScoreBytes / row_bytes : heads;
+    if (pass < 1) pass = 1;
+    const size_t score_bytes = scored ? row_bytes * pass : 0;
+    S3DSP_CUDA(malloc_async(&means, (n_qm + n_km) * sizeof(double) + score_bytes + 16, ctx->stream), "block scores");
     MeanParams m = {q, k, q_stride, k_stride, (int)qw, (int)kw, plan->n_qb, plan->n_kb, plan->q_blocks, plan->k_blocks,
                     means, means + n_qm};
     const bool vec = !(((uintptr_t)q | (uintptr_t)k | (q_stride * es) | (k_stride * es)) & 15);
     const dim3 mg((unsigned)(plan->n_qb + plan->n_kb), (unsigned)ceil_div(qw, kMeanCols));
     cudaError_t e = cudaSuccess;
     auto mean = [&](auto kernel) { e = launch_pdl(kernel, mg, dim3(kMeanThreads), 0, ctx->stream, m); };
-    if (dtype == S3DSP_F32)
+    if (!scored)
+        ;  // every list holds all blocks
+    else if (dtype == S3DSP_F32)
         vec ? mean(block_mean_kernel<float, true>) : mean(block_mean_kernel<float, false>);
     else if (dtype == S3DSP_BF16)
         vec ? mean(block_mean_kernel<__nv_bfloat16, true>) : mean(block_mean_kernel<__nv_bfloat16, false>);
     else
         vec ? mean(block_mean_kernel<__half, true>) : mean(block_mean_kernel<__half, false>);
-    if (e == cudaSuccess) {
-        ScoreParams s = {plan->groups, plan->q_blocks, plan->first_kb, means, means + n_qm, (int)qw, plan->n_kb, d, heads,
-                         heads / kv_heads, top, keep_local, plan->max_kb, d_sel};
-        e = launch_pdl(block_score_kernel, dim3((unsigned)plan->n_groups, (unsigned)heads), dim3(kScoreThreads), smem,
-                       ctx->stream, s);
+    ScoreParams s = {plan->groups, plan->q_blocks, plan->first_kb, means, means + n_qm, (int)qw, (int)kw, plan->n_qb, d,
+                     heads, heads / kv_heads, top, keep_local, 0, 0, plan->max_kb,
+                     reinterpret_cast<unsigned long long*>(means + n_qm + n_km), d_sel};
+    for (int h0 = 0; h0 < heads && e == cudaSuccess; h0 += (int)pass) {
+        s.head0 = h0;
+        s.head_count = (int)(heads - h0 < pass ? heads - h0 : pass);
+        if (scored)
+            e = launch_pdl(block_score_kernel,
+                           dim3((unsigned)plan->n_groups, (unsigned)ceil_div(plan->max_kb, kTileK), (unsigned)s.head_count),
+                           dim3(kScoreThreads), 0, ctx->stream, s);
+        if (e != cudaSuccess) break;
+        const int64_t items = (int64_t)plan->n_qb * s.head_count;
+        if (plan->max_kb <= 32 * kWarpKeys)
+            e = launch_pdl(top_warp_kernel, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, ctx->stream, s);
+        else
+            e = launch_pdl(top_block_kernel, dim3((unsigned)items), dim3(kTopThreads),
+                           (plan->max_kb + 1) * sizeof(unsigned long long), ctx->stream, s);
     }
     const cudaError_t f = cudaFreeAsync(means, ctx->stream);
     if (e == cudaSuccess) e = f;

@@ -84,16 +84,14 @@ struct s3dsp_attn_plan {
     int device = 0;
     bool self = false;               // the key rows are the query rows
     int64_t n_q = 0, n_k = 0;        // rows the plan spans (the last offsets)
-    int64_t first_q = 0;             // first query row of the first sequence
     int64_t sum_kb = 0;              // over the query blocks: their sequence's key blocks
     int max_q_rows = 0;              // most rows of a query block
     int n_qb = 0, n_kb = 0, n_groups = 0;
     int max_kb = 0;                  // most key blocks of a sequence
-    int group = 1;                   // query blocks of a selection group
     void* mem = nullptr;
     int4* q_blocks = nullptr;        // [n_qb] {first row, rows | index in the sequence << 8, first key row, key rows}
     int2* k_blocks = nullptr;        // [n_kb] {first row, rows}
-    int2* groups = nullptr;          // [n_groups] {first query block, up to `group` blocks of one sequence}
+    int2* groups = nullptr;          // [n_groups] {first query block, up to kAttnGroupRows blocks of one sequence}
     int* first_kb = nullptr;         // [n_qb] first key block of the block's sequence
 };
 
@@ -103,7 +101,7 @@ constexpr int kAttnQRows = 128;      // rows of a query block (tcgen05 M)
 constexpr int kAttnKRows = 64;       // rows of a key block
 constexpr int kAttnRowsBits = 8;     // s3dsp_attn_plan::q_blocks[].y: rows below, index above
 constexpr int kAttnRowsMask = (1 << kAttnRowsBits) - 1;
-constexpr int kAttnGroupRows = 16;   // most query blocks whose block scores are computed together
+constexpr int kAttnGroupRows = 32;   // query blocks whose block scores are computed together
 constexpr int kAttnMaxTop = 1024;    // longest list of key blocks
 
 constexpr int kTileRows = 128;  // rows per conv tile (tcgen05 M) == tile_mask granularity

@@ -375,6 +375,12 @@ ATTEND = [
     ([4000], None, 2, 2, 64, 16, 0),
     ([260], [9000], 2, 1, 64, 0, 0),
     ([50], [20000], 2, 1, 128, 0, 0),
+    ([2600, 129], [600, 3000], 16, 8, 64, 0, 0),     # tiles for more than a wave
+    ([2600, 129], [600, 3000], 16, 16, 128, 7, 0),
+    ([128 * 19, 50], [64 * 30, 64 * 60], 16, 16, 64, 0, 0),  # a wave of whole tiles, then shared ones
+    ([128 * 19, 50], [64 * 30, 64 * 60], 16, 4, 128, 40, 0),
+    ([7, 1, 30], [3000, 200, 5000], 12, 2, 64, 0, 0),  # groups of 6: tiles of 2 heads
+    ([7, 1, 3], [3000, 0, 5000], 32, 1, 128, 0, 0),    # 16 heads a tile
 ]
 
 
