@@ -27,8 +27,9 @@ namespace {
 
 constexpr int kMeanThreads = 256;
 constexpr int kMeanCols = 256;  // columns per CTA of the mean kernel: 32 lanes x 8
-constexpr int kScoreThreads = 128;
-constexpr int kTileQ = kAttnGroupRows, kTileK = 64, kTileD = 32;  // of the score kernel
+constexpr int kTileQ = kAttnGroupRows, kTileK = 128, kTileD = 32;  // of the score kernel
+constexpr int kScoreThreads = 32 * (kTileK / 32);                    // a warp per 32 key blocks
+constexpr int kScoreLd = kTileD + 4;                                // shared row: 8 rows x 4 columns hit every bank once
 constexpr int kWarpKeys = 32;                                     // key blocks per lane of top_warp_kernel
 constexpr int kMaxKeys = 28000;                                   // key blocks of a sequence: top_block_kernel's memory
 constexpr size_t kScoreBytes = (size_t)1 << 29;                   // scratch of scores that a pass over heads may take
@@ -136,10 +137,19 @@ __device__ __forceinline__ unsigned long long ordered(double v) {
     return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-// A thread owns 4 query blocks x 4 key blocks; every score is summed over the
-// head's columns in order, so that equal blocks have equal scores.
+// d (8 x 8, two values a lane) += a (8 x 4) b^T (8 x 4), f64
+__device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
+    asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                 : "+d"(d[0]), "+d"(d[1])
+                 : "d"(a), "d"(b));
+}
+
+// A warp owns 32 query blocks x 32 key blocks as 4 x 4 f64 MMAs: eight shared
+// loads feed sixteen of them. (Scalar FMAs run at the same rate but need a
+// shared load each: 90 us with 4 x 4 register blocks where this takes 46.) Every
+// score is the same sequence of MMA steps, so that equal blocks have equal scores.
 __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreParams p) {
-    __shared__ __align__(16) double qs[kTileD][kTileQ + 2], ks[kTileD][kTileK + 2];
+    __shared__ __align__(16) double qs[kTileQ][kScoreLd], ks[kTileK][kScoreLd];
     pdl_wait();
     pdl_trigger();
     const int2 grp = p.groups[blockIdx.x];
@@ -147,50 +157,58 @@ __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreP
     const int4 qb0 = p.q_blocks[b0];
     const int nkb = (qb0.w + kAttnKRows - 1) / kAttnKRows;
     if (c0 >= nkb || nkb <= p.top) return;  // all blocks are taken: no scores needed
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lr = lane >> 2, lk = lane & 3;  // the lane's row and column of an operand
     const double* qm = p.q_mean + (int64_t)b0 * p.qw + (int64_t)h * p.d;
     const double* km = p.k_mean + (int64_t)(p.first_kb[b0] + c0) * p.kw + (int64_t)(h / p.per_kv) * p.d;
-    double acc[4][4];
+    double acc[4][4][2];
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[x][y] = 0.0;
+        for (int y = 0; y < 4; ++y) acc[x][y][0] = acc[x][y][1] = 0.0;
+    const bool work = c0 + 32 * warp < nkb;
     for (int j0 = 0; j0 < p.d; j0 += kTileD) {
-        const int dn = min(kTileD, p.d - j0);
-        const int j = threadIdx.x & (kTileD - 1);
+        const int j = 2 * (threadIdx.x % (kTileD / 2)), r0 = threadIdx.x / (kTileD / 2);
+        constexpr int kStep = kScoreThreads / (kTileD / 2);
+        const double2 zero = make_double2(0.0, 0.0);  // d is a multiple of 8
 #pragma unroll
-        for (int r = threadIdx.x / kTileD; r < kTileQ; r += kScoreThreads / kTileD)
-            qs[j][r] = r < count && j < dn ? qm[(int64_t)r * p.qw + j0 + j] : 0.0;
-#pragma unroll
-        for (int c = threadIdx.x / kTileD; c < kTileK; c += kScoreThreads / kTileD)
-            ks[j][c] = c0 + c < nkb && j < dn ? km[(int64_t)c * p.kw + j0 + j] : 0.0;
+        for (int r = r0; r < kTileQ; r += kStep)
+            *reinterpret_cast<double2*>(&qs[r][j]) =
+                r < count && j0 + j < p.d ? *reinterpret_cast<const double2*>(qm + (int64_t)r * p.qw + j0 + j) : zero;
+#pragma unroll 8
+        for (int c = r0; c < kTileK; c += kStep)
+            *reinterpret_cast<double2*>(&ks[c][j]) =
+                c0 + c < nkb && j0 + j < p.d ? *reinterpret_cast<const double2*>(km + (int64_t)c * p.kw + j0 + j) : zero;
         __syncthreads();
-#pragma unroll 4
-        for (int i = 0; i < dn; ++i) {
-            const double2 q01 = *reinterpret_cast<const double2*>(&qs[i][4 * ty]);
-            const double2 q23 = *reinterpret_cast<const double2*>(&qs[i][4 * ty + 2]);
-            const double2 k01 = *reinterpret_cast<const double2*>(&ks[i][2 * tx]);
-            const double2 k23 = *reinterpret_cast<const double2*>(&ks[i][2 * tx + 32]);
-            const double qv[4] = {q01.x, q01.y, q23.x, q23.y}, kv[4] = {k01.x, k01.y, k23.x, k23.y};
+        if (work) {
+#pragma unroll 2
+            for (int i = 0; i < kTileD; i += 4) {
+                double a[4], b[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+                for (int x = 0; x < 4; ++x) a[x] = qs[8 * x + lr][i + lk], b[x] = ks[32 * warp + 8 * x + lr][i + lk];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) acc[x][y] = fma(qv[x], kv[y], acc[x][y]);
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) mma_f64(acc[x][y], a[x], b[y]);
+            }
         }
         __syncthreads();
     }
+    if (!work) return;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-        const int r = 4 * ty + x;
-        if (r >= count) break;
+        const int r = 8 * x + lr;
+        if (r >= count) continue;
         // the key blocks of the query block's own rows come first
         const int own = p.keep_local ? ((qb0.y >> kAttnRowsBits) + r) * (kAttnQRows / kAttnKRows) : -2;
         unsigned long long* row = p.keys + ((int64_t)(b0 + r) * p.head_count + blockIdx.z) * p.max_kb;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-            const int c = c0 + 2 * tx + (y & 1) + 32 * (y >> 1);
-            if (c < nkb) row[c] = c >= own && c < own + kAttnQRows / kAttnKRows ? ~0ull : ordered(acc[x][y]);
-        }
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = c0 + 32 * warp + 8 * y + 2 * lk + e;
+                if (c < nkb) row[c] = c >= own && c < own + kAttnQRows / kAttnKRows ? ~0ull : ordered(acc[x][y][e]);
+            }
     }
 }
 
@@ -205,7 +223,9 @@ __device__ __forceinline__ void emit(int32_t* out, int c, bool above, bool equal
     ties -= min(ties, __popc(em));
 }
 
+constexpr int kCandidates = 128;
 __global__ void __launch_bounds__(128) top_warp_kernel(const ScoreParams p) {
+    __shared__ int candidates[4][kCandidates];
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
@@ -232,17 +252,90 @@ __global__ void __launch_bounds__(128) top_warp_kernel(const ScoreParams p) {
             hi_bound = max(hi_bound, hi[i]);
         }
     }
-    // the largest t with at least `top` upper halves >= t: count(lo) >= top > count(up)
-    uint32_t lo = __reduce_min_sync(0xffffffffu, lo_bound);
+    // lo: at_lo >= top upper halves are >= lo; up: fewer are >= up. For up to 32
+    // blocks the top-th largest of the lanes' maxima is such an lo, close to the
+    // threshold (each lane holds every 32nd block).
+    const uint32_t low = __reduce_min_sync(0xffffffffu, lo_bound);
     uint64_t up = (uint64_t)__reduce_max_sync(0xffffffffu, hi_bound) + 1;
-    int at_lo = nkb;
-    while (up - lo > 1 && at_lo != p.top) {
-        const uint32_t mid = (uint32_t)(lo + (up - lo) / 2);
+    uint32_t lo = low;
+    if (p.top <= 32) {
+        int rank = 0;
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+            const uint32_t other = __shfl_sync(0xffffffffu, hi_bound, x);
+            rank += other > hi_bound || (other == hi_bound && x < lane);
+        }
+        const unsigned m = __ballot_sync(0xffffffffu, rank == p.top - 1);
+        lo = max(low, __shfl_sync(0xffffffffu, hi_bound, __ffs(m) - 1));
+    }
+    auto count = [&](uint32_t t) {
         int m = 0;
 #pragma unroll
         for (int i = 0; i < kWarpKeys; ++i)
-            if (i < steps) m += hi[i] >= mid;  // the padding's 0 is below every mid > lo >= 0
-        m = __reduce_add_sync(0xffffffffu, m);
+            if (i < steps) m += 32 * i + lane < nkb && hi[i] >= t;
+        return (int)__reduce_add_sync(0xffffffffu, m);
+    };
+    int at_lo = count(lo);
+    while (up - lo > 1 && at_lo > kCandidates) {
+        const uint32_t mid = (uint32_t)(lo + (up - lo) / 2);
+        const int m = count(mid);
+        if (m >= p.top)
+            lo = mid, at_lo = m;
+        else
+            up = mid;
+    }
+    if (at_lo <= kCandidates) {
+        // the blocks left, in index order, four to a lane; their whole keys decide
+        int* cand = candidates[threadIdx.x >> 5];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kWarpKeys; ++i)
+            if (i < steps) {
+                const bool is = 32 * i + lane < nkb && hi[i] >= lo;
+                const unsigned m = __ballot_sync(0xffffffffu, is);
+                if (is) cand[n + __popc(m & ((1u << lane) - 1u))] = 32 * i + lane;
+                n += __popc(m);
+            }
+        __syncwarp();
+        const unsigned long long* key64 = p.keys + item * p.max_kb;
+        unsigned long long k[kCandidates / 32];
+        int c[kCandidates / 32];
+#pragma unroll
+        for (int i = 0; i < kCandidates / 32; ++i) {
+            const bool is = 32 * i + lane < n;
+            c[i] = is ? cand[32 * i + lane] : -1;
+            k[i] = is ? key64[c[i]] : 0ull;
+        }
+        unsigned long long a = (unsigned long long)lo << 32;
+        unsigned long long z = up > 0xffffffffull ? ~0ull : ((unsigned long long)up << 32) - 1;  // no key is above z
+        // the largest threshold in [a, z] that `top` keys reach
+        int at_a = n;
+        while (a < z && at_a != p.top) {
+            const unsigned long long mid = a + (z - a) / 2 + 1;
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < kCandidates / 32; ++i) m += c[i] >= 0 && k[i] >= mid;
+            m = __reduce_add_sync(0xffffffffu, m);
+            if (m >= p.top)
+                a = mid, at_a = m;
+            else
+                z = mid - 1;
+        }
+        int over = 0, done = 0;
+#pragma unroll
+        for (int i = 0; i < kCandidates / 32; ++i) over += c[i] >= 0 && k[i] > a;
+        int ties = p.top - (int)__reduce_add_sync(0xffffffffu, over);
+        if (at_a == p.top) ties = n;  // all that reach it
+#pragma unroll
+        for (int i = 0; i < kCandidates / 32; ++i)
+            if (32 * i < n) emit(out, c[i], c[i] >= 0 && k[i] > a, c[i] >= 0 && k[i] == a, lane, done, ties);
+        return;
+    }
+    // lists longer than that, or as many keys that share the threshold's upper
+    // half (up = lo + 1): bisect on
+    while (up - lo > 1 && at_lo != p.top) {
+        const uint32_t mid = (uint32_t)(lo + (up - lo) / 2);
+        const int m = count(mid);
         if (m >= p.top)
             lo = mid, at_lo = m;
         else

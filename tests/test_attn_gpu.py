@@ -274,6 +274,35 @@ def test_block_select_ties_and_nan(ctx):
     assert (sel.cpu().numpy() == np.arange(top)).all()
 
 
+@pytest.mark.parametrize("copies", [3, 40])
+@pytest.mark.parametrize("n", [64 * 50, 64 * 900, 64 * 1500])
+def test_block_select_equal_blocks(ctx, n, copies):
+    """Copies of one key block anywhere have one score, bit by bit: the first of them are taken."""
+    q, k = randn((600, 128), 1, torch.bfloat16), randn((n, 128), 2, torch.bfloat16)
+    g = np.random.default_rng(n + copies)
+    at = np.sort(g.permutation(n // 64)[:copies])
+    for c in at[1:]:
+        k[64 * c:64 * c + 64] = k[64 * at[0]:64 * at[0] + 64]
+    plan = ctx.attn_plan([0, 600], [0, n])
+    for top in (1, 9, copies, 45):
+        sel = torch.empty((plan.q_blocks, 2, top), dtype=torch.int32, device="cuda")
+        ctx.block_select(plan, q, k, 2, 2, sel)
+        for row in sel.reshape(-1, top).cpu().numpy():
+            taken = np.isin(at, row)
+            assert taken[:taken.sum()].all(), (at, row)
+        assert (sel[..., 1:] > sel[..., :-1]).all()
+
+
+@pytest.mark.parametrize("top", [1, 31, 33, 64, 129, 500])
+@pytest.mark.parametrize("n", [64 * 640, 64 * 1100])
+def test_block_select_list_lengths(ctx, n, top):
+    q, k = randn((300, 128), 3, torch.bfloat16), randn((n, 128), 4, torch.bfloat16)
+    plan = ctx.attn_plan([0, 300], [0, n])
+    sel = torch.empty((plan.q_blocks, 2, top), dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, 2, 2, sel)
+    assert torch.equal(sel.cpu(), chosen(q, k, [300], [n], 2, 2, top, False))
+
+
 @pytest.mark.parametrize("n", [120000, 300000])
 def test_block_select_long_sequence(ctx, n):
     """More key blocks than sixteen score rows leave room for (groups of fewer query blocks)."""
