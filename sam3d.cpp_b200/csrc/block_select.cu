@@ -27,10 +27,11 @@ namespace {
 
 constexpr int kMeanThreads = 256;
 constexpr int kMeanCols = 256;  // columns per CTA of the mean kernel: 32 lanes x 8
-constexpr int kTileQ = kAttnGroupRows, kTileK = 128, kTileD = 32;  // of the score kernel
+constexpr int kTileQ = kAttnGroupRows, kTileK = 128, kTileD = 16;  // of the score kernel
 constexpr int kScoreThreads = 32 * (kTileK / 32);                    // a warp per 32 key blocks
 constexpr int kScoreLd = kTileD + 4;                                // shared row: 8 rows x 4 columns hit every bank once
 constexpr int kWarpKeys = 32;                                     // key blocks per lane of top_warp_kernel
+constexpr size_t kScoreSmem = 2 * sizeof(double) * (kTileQ + kTileK) * kScoreLd;  // four CTAs per SM
 constexpr int kMaxKeys = 28000;                                   // key blocks of a sequence: top_block_kernel's memory
 constexpr size_t kScoreBytes = (size_t)1 << 29;                   // scratch of scores that a pass over heads may take
 
@@ -88,21 +89,28 @@ __global__ void __launch_bounds__(kMeanThreads) block_mean_kernel(MeanParams p) 
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.0;
     if (c < width) {  // widths are multiples of 8
-#pragma unroll 4
-        for (int r = warp; r < rows; r += 8) {
-            const T* x = base + r * ld;
-            T e[8];
-            if constexpr (kVec) {
-                constexpr int kW = sizeof(T) * 8 / 16;
+        constexpr int U = sizeof(T) == 4 ? 4 : 8;  // rows in flight
+        for (int r0 = warp; r0 < rows; r0 += 8 * U) {
+            T e[U][8];
 #pragma unroll
-                for (int w = 0; w < kW; ++w)
-                    reinterpret_cast<uint4*>(e)[w] = __ldg(reinterpret_cast<const uint4*>(x) + w);
-            } else {
+            for (int u = 0; u < U; ++u) {
+                const T* x = base + (int64_t)(r0 + 8 * u) * ld;
+                if (r0 + 8 * u >= rows) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = x[j];
+                    for (int j = 0; j < 8; ++j) e[u][j] = T(0.f);
+                } else if constexpr (kVec) {
+#pragma unroll
+                    for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+                        reinterpret_cast<uint4*>(e[u])[w] = __ldg(reinterpret_cast<const uint4*>(x) + w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e[u][j] = x[j];
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += to_d(e[j]);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] += to_d(e[u][j]);
         }
     }
 #pragma unroll
@@ -149,7 +157,8 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
 // shared load each: 90 us with 4 x 4 register blocks where this takes 46.) Every
 // score is the same sequence of MMA steps, so that equal blocks have equal scores.
 __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreParams p) {
-    __shared__ __align__(16) double qs[kTileQ][kScoreLd], ks[kTileK][kScoreLd];
+    // two stages of kTileD columns of the query rows and, below them, the key rows
+    extern __shared__ __align__(16) double stage[][kTileQ + kTileK][kScoreLd];
     pdl_wait();
     pdl_trigger();
     const int2 grp = p.groups[blockIdx.x];
@@ -167,25 +176,32 @@ __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreP
 #pragma unroll
         for (int y = 0; y < 4; ++y) acc[x][y][0] = acc[x][y][1] = 0.0;
     const bool work = c0 + 32 * warp < nkb;
-    for (int j0 = 0; j0 < p.d; j0 += kTileD) {
-        const int j = 2 * (threadIdx.x % (kTileD / 2)), r0 = threadIdx.x / (kTileD / 2);
-        constexpr int kStep = kScoreThreads / (kTileD / 2);
-        const double2 zero = make_double2(0.0, 0.0);  // d is a multiple of 8
+    // rows or columns that are not there: zeros (d is a multiple of 8)
+    auto load = [&](int j0, int st) {
+        const int j = 2 * (threadIdx.x % (kTileD / 2));
 #pragma unroll
-        for (int r = r0; r < kTileQ; r += kStep)
-            *reinterpret_cast<double2*>(&qs[r][j]) =
-                r < count && j0 + j < p.d ? *reinterpret_cast<const double2*>(qm + (int64_t)r * p.qw + j0 + j) : zero;
-#pragma unroll 8
-        for (int c = r0; c < kTileK; c += kStep)
-            *reinterpret_cast<double2*>(&ks[c][j]) =
-                c0 + c < nkb && j0 + j < p.d ? *reinterpret_cast<const double2*>(km + (int64_t)c * p.kw + j0 + j) : zero;
+        for (int r = threadIdx.x / (kTileD / 2); r < kTileQ + kTileK; r += kScoreThreads / (kTileD / 2)) {
+            const bool q = r < kTileQ, in = j0 + j < p.d && (q ? r < count : c0 + r - kTileQ < nkb);
+            const double* src = q ? qm + (int64_t)r * p.qw : km + (int64_t)(r - kTileQ) * p.kw;
+            const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&stage[st][r][j]);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? src + j0 + j : qm),
+                         "r"(in ? 16 : 0)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    load(0, 0);
+    for (int j0 = 0, st = 0; j0 < p.d; j0 += kTileD, st ^= 1) {
+        load(j0 + kTileD, st ^ 1);  // past the last column: zeros that nothing reads
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncthreads();
         if (work) {
-#pragma unroll 2
+#pragma unroll
             for (int i = 0; i < kTileD; i += 4) {
                 double a[4], b[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) a[x] = qs[8 * x + lr][i + lk], b[x] = ks[32 * warp + 8 * x + lr][i + lk];
+                for (int x = 0; x < 4; ++x)
+                    a[x] = stage[st][8 * x + lr][i + lk], b[x] = stage[st][kTileQ + 32 * warp + 8 * x + lr][i + lk];
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -194,6 +210,7 @@ __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreP
         }
         __syncthreads();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!work) return;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -576,7 +593,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "a sequence has %d key blocks (at most %d)",
                     plan->max_kb, kMaxKeys);
     S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
-    static std::atomic<uint64_t> optin{0};
+    static std::atomic<uint64_t> optin{0}, score_optin{0};
+    S3DSP_CUDA(smem_optin((const void*)block_score_kernel, ctx->device, score_optin), "block_score_kernel");
     S3DSP_CUDA(smem_optin((const void*)top_block_kernel, ctx->device, optin), "top_block_kernel");
     double* means = nullptr;
     const size_t n_qm = (size_t)plan->n_qb * qw, n_km = (size_t)plan->n_kb * kw;
@@ -610,7 +628,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
         if (scored)
             e = launch_pdl(block_score_kernel,
                            dim3((unsigned)plan->n_groups, (unsigned)ceil_div(plan->max_kb, kTileK), (unsigned)s.head_count),
-                           dim3(kScoreThreads), 0, ctx->stream, s);
+                           dim3(kScoreThreads), kScoreSmem, ctx->stream, s);
         if (e != cudaSuccess) break;
         const int64_t items = (int64_t)plan->n_qb * s.head_count;
         if (plan->max_kb <= 32 * kWarpKeys)
