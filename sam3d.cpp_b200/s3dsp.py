@@ -14,7 +14,9 @@ S3dError carrying both.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libs3dsp.so")
@@ -216,9 +218,19 @@ def load(path: str = LIB_PATH):
     return L
 
 
+class _ErrorBuffer(threading.local):
+    """Each thread's error buffer: a call fills it only when it fails."""
+
+    def __init__(self):
+        self.buf = ctypes.create_string_buffer(512)
+
+
+_error = _ErrorBuffer()
+
+
 def _call(fn, *args):
-    buf = ctypes.create_string_buffer(512)
-    st = fn(*args, buf, ctypes.c_uint64(len(buf)))
+    buf = _error.buf
+    st = fn(*args, buf, 512)
     if st != S3D_OK:
         raise S3dError(st, buf.value.decode(errors="replace"))
 
@@ -230,27 +242,40 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_codes: dict = {}
+
+
 def dtype_code(t) -> int:
-    import torch
-    return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}[t.dtype]
+    if not _codes:
+        import torch
+        _codes.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    return _codes[t.dtype]
+
+
+@functools.lru_cache(maxsize=64)
+def _int32s(values: tuple):
+    """A host int32 array (the same values are built once)."""
+    return (_i32 * len(values))(*values)
 
 
 def _rows(t, name: str):
     """(address, row stride) of a 2-D tensor whose columns are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: rows of contiguous columns are wanted")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]))
+    return t.data_ptr(), (stride[0] if shape[0] > 1 else max(stride[0], shape[1]))
 
 
 def _head_dim(t, heads: int, name: str) -> int:
-    if heads <= 0 or t.shape[1] % heads:
-        raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: {t.shape[1]} columns are no {heads} heads")
-    return t.shape[1] // heads
+    w = t.shape[-1]
+    if heads <= 0 or w % heads:
+        raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: {w} columns are no {heads} heads")
+    return w // heads
 
 
-def _same(what: str, *vals):
-    if any(v != vals[0] for v in vals[1:]):
-        raise S3dError(S3D_INVALID_ARGUMENT, f"{what} differ: {vals}")
+def _same(what: str, a, b):
+    if a != b:
+        raise S3dError(S3D_INVALID_ARGUMENT, f"{what} differ: {a}, {b}")
 
 
 class Kmap:
@@ -665,35 +690,34 @@ class Context:
     @staticmethod
     def _positions(positions, axis_pairs, n):
         """(address, row stride, axes, host axis_pairs) of int32 positions [n, >= axes]."""
-        import torch
         axes = len(axis_pairs)
         if axes == 0:
             return None, 0, 0, None
-        if positions is None or positions.dim() != 2 or positions.dtype != torch.int32 or positions.shape[0] != n \
-                or positions.shape[1] < axes or (positions.shape[1] > 1 and positions.stride(1) != 1):
+        import torch
+        if positions is None or positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[0] != n \
+                or positions.shape[1] < axes:
             raise S3dError(S3D_INVALID_ARGUMENT, f"positions: int32 [{n}, >= {axes}] rows are wanted")
-        stride = positions.stride(0) if n > 1 else max(positions.stride(0), positions.shape[1])
-        return positions.data_ptr(), stride, axes, (_i32 * axes)(*axis_pairs)
+        return *_rows(positions, "positions"), axes, _int32s(tuple(axis_pairs))
 
     def rope(self, x, positions, heads: int, out, axis_pairs, theta: float = 10000.0, half: bool = False,
              inverse: bool = False):
         """out = x [n, heads * d] with every head turned by positions (int32
         [n, axes]); axis_pairs: pairs of each axis. Rows may be strided."""
         d = _head_dim(x, heads, "x")
-        _same("x and out", tuple(x.shape), tuple(out.shape))
+        _same("x and out", x.shape, out.shape)
+        n = x.shape[0]
         xp, xs = _rows(x, "x")
         yp, ys = _rows(out, "out")
-        pos, pst, axes, pairs = self._positions(positions, axis_pairs, x.shape[0])
-        _call(load().s3dsp_rope, self.handle, xp, dtype_code(x), x.shape[0], xs, heads, d, pos, pst, axes, pairs, theta,
+        pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
+        _call(load().s3dsp_rope, self.handle, xp, dtype_code(x), n, xs, heads, d, pos, pst, axes, pairs, theta,
               (ROPE_HALF if half else 0) | (ROPE_INVERSE if inverse else 0), yp, dtype_code(out), ys)
 
     def qk_norm_rope(self, q, heads: int, q_gamma, q_out, k=None, kv_heads: int = 0, k_gamma=None, k_out=None,
                      eps: float = 1e-6, positions=None, axis_pairs=(), theta: float = 10000.0, half: bool = False):
         """RMS norm of every head of q (and k) with weights f32 [heads, d] (or
         [d] for all heads, or None), then the rotation (axis_pairs () : none)."""
-        import torch
         n, d = q.shape[0], _head_dim(q, heads, "q")
-        _same("q and q_out", tuple(q.shape), tuple(q_out.shape))
+        _same("q and q_out", q.shape, q_out.shape)
         qp, qs = _rows(q, "q")
         qop, qos = _rows(q_out, "q_out")
         kp = kop = None
@@ -701,21 +725,29 @@ class Context:
         flags = ROPE_HALF if half else 0
         if k is not None:
             _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
-            _same("rows and types", (n, q.dtype), (k.shape[0], k.dtype))
-            _same("k and k_out", tuple(k.shape), tuple(k_out.shape))
+            _same("rows of q and k", n, k.shape[0])
+            _same("types of q and k", q.dtype, k.dtype)
+            _same("k and k_out", k.shape, k_out.shape)
             _same("output types", q_out.dtype, k_out.dtype)
             kp, ks = _rows(k, "k")
             kop, kos = _rows(k_out, "k_out")
-        gammas = [(g, h) for g, h in ((q_gamma, heads), (k_gamma, kv_heads)) if g is not None]
-        if any(g.dim() == 1 for g, _ in gammas):
+        if (q_gamma is not None and q_gamma.dim() == 1) or (k_gamma is not None and k_gamma.dim() == 1):
             flags |= QK_GAMMA_SHARED
-        for g, h in gammas:
-            want = (d,) if flags & QK_GAMMA_SHARED else (h, d)
-            if tuple(g.shape) != want or g.dtype != torch.float32 or not g.is_contiguous():
-                raise S3dError(S3D_INVALID_ARGUMENT, f"gamma: contiguous float32 {want} is wanted")
         pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
-        _call(load().s3dsp_qk_norm_rope, self.handle, qp, qs, heads, ptr(q_gamma), kp, ks, kv_heads, ptr(k_gamma),
-              dtype_code(q), n, d, eps, pos, pst, axes, pairs, theta, flags, qop, qos, kop, kos, dtype_code(q_out))
+        _call(load().s3dsp_qk_norm_rope, self.handle, qp, qs, heads, self._gamma(q_gamma, heads, d, flags), kp, ks,
+              kv_heads, self._gamma(k_gamma, kv_heads, d, flags), dtype_code(q), n, d, eps, pos, pst, axes, pairs, theta,
+              flags, qop, qos, kop, kos, dtype_code(q_out))
+
+    @staticmethod
+    def _gamma(g, heads: int, d: int, flags: int):
+        """Address of a norm weight: f32 [heads, d], or [d] when shared."""
+        if g is None:
+            return None
+        want = (d,) if flags & QK_GAMMA_SHARED else (heads, d)
+        import torch
+        if g.dtype != torch.float32 or tuple(g.shape) != want or not g.is_contiguous():
+            raise S3dError(S3D_INVALID_ARGUMENT, f"gamma: contiguous float32 {want} is wanted")
+        return g.data_ptr()
 
     def attn_plan(self, q_offsets, k_offsets=None) -> AttnPlan:
         """Plan of a ragged batch: host offsets [n_seq + 1] of the sequences'
@@ -739,31 +771,34 @@ class Context:
             raise S3dError(S3D_INVALID_ARGUMENT, f"the plan spans {plan.n_q} query rows and {plan.n_k} key rows")
         return d
 
+    @staticmethod
+    def _lists(sel, plan: AttnPlan, heads: int) -> int:
+        """The length of the lists in sel (int32 [plan.q_blocks, heads, top])."""
+        import torch
+        shape = sel.shape
+        if len(shape) != 3 or shape[0] != plan.q_blocks or shape[1] != heads or sel.dtype != torch.int32 or \
+                not sel.is_contiguous():
+            raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
+        return shape[2]
+
     def block_select(self, plan: AttnPlan, q, k, heads: int, kv_heads: int, sel, keep_local: bool = False):
         """sel (device int32 [plan.q_blocks, heads, top]) = the key blocks with the largest scores."""
-        import torch
         d = self._attn_rows(plan, q, heads, k, kv_heads)
-        if sel.dim() != 3 or sel.dtype != torch.int32 or not sel.is_contiguous() or \
-                tuple(sel.shape[:2]) != (plan.q_blocks, heads):
-            raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
+        top = self._lists(sel, plan, heads)
         qp, qs = _rows(q, "q")
         kp, ks = _rows(k, "k")
         _call(load().s3dsp_block_select, self.handle, plan.handle, qp, qs, heads, kp, ks, kv_heads, dtype_code(q), d,
-              sel.shape[2], int(keep_local), ptr(sel))
+              top, int(keep_local), sel.data_ptr())
 
     def block_attention(self, plan: AttnPlan, q, k, v, heads: int, kv_heads: int, out, scale: float | None = None,
                         sel=None):
         """out = softmax(scale q k^T over the listed key blocks (sel None: all)) v; scale None: 1 / sqrt(d)."""
-        import torch
         d = self._attn_rows(plan, q, heads, k, kv_heads)
-        _same("k and v", (tuple(k.shape), k.dtype), (tuple(v.shape), v.dtype))
-        _same("q and out", (tuple(q.shape), q.dtype), (tuple(out.shape), out.dtype))
-        top = 0
-        if sel is not None:
-            if sel.dim() != 3 or sel.dtype != torch.int32 or not sel.is_contiguous() or \
-                    tuple(sel.shape[:2]) != (plan.q_blocks, heads):
-                raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
-            top = sel.shape[2]
+        _same("k and v", k.shape, v.shape)
+        _same("q and out", q.shape, out.shape)
+        if not q.dtype == v.dtype == out.dtype:
+            raise S3dError(S3D_INVALID_ARGUMENT, f"types of q, v and out differ: {q.dtype}, {v.dtype}, {out.dtype}")
+        top = 0 if sel is None else self._lists(sel, plan, heads)
         (qp, qs), (kp, ks), (vp, vs), (op, os_) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
         _call(load().s3dsp_block_attention, self.handle, plan.handle, qp, qs, heads, kp, ks, vp, vs, kv_heads,
               dtype_code(q), d, d ** -0.5 if scale is None else scale, ptr(sel), top, op, os_)
