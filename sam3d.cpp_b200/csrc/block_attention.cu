@@ -3,34 +3,37 @@
 //
 // One CTA per (query block of 128 rows, head); short blocks of grouped heads
 // share a tile, and where there are few tiles their lists are split over CTAs
-// and joined by a second kernel. The row maximum and sum run
-// along with the blocks (online softmax), so scores never leave the SM:
+// and joined by a second kernel. The row maximum and sum run along with the
+// blocks (online softmax), so scores never leave the SM:
 //
-//   producer warp   TMA: the Q tile once, then the K and V tiles of the listed blocks into rings
-//   MMA warp        S = Q K^T (tcgen05, f32 in TMEM), then O += P V with P read from TMEM
-//   softmax warps   one thread per query row: S from TMEM, running maximum, p = 2^(c s - c m),
-//                   running sum, P back into S's columns
+//   key warp        K tiles by TMA into a ring; S = Q K^T (tcgen05, f32 in TMEM)
+//   value warp      V tiles by TMA into a ring; O += P V with P read from TMEM
+//   softmax warps   one thread per query row: S from TMEM, p = 2^(c s - c m), maximum and sum on the
+//                   way, P back into S's first columns
 //
-// kBufs score buffers: the scores of the next blocks are computed while this
+// Two score buffers: the scores of the next block are computed while this
 // block's softmax runs, and P(j) V(j) while softmax(j + 1) runs, so that the
-// softmax warps wait for neither. P(j) takes the first columns of S(j); Q K^T
-// writes a buffer again only after P V, its last reader, has completed.
+// softmax warps wait for neither. Q K^T writes a buffer again only after P V,
+// its last reader, has completed.
 //
-// What bounds it (one B200; us per 128 x 64 tile and SM, dense 4096^2 rows):
-//   d = 64   0.434 (715 TFLOP/s): without the exponentials 0.34, without MMAs 0.40, MMAs and barriers
-//            alone 0.29. Two softmax warps per scheduler issue in 54 % of the cycles, the tensor pipe is
-//            busy in 48 %: the chain of a softmax step (score load, maximum, exponentials, P store). More
-//            warps did not help: two groups or two threads per row, or four CTAs per SM, took 0.44 - 0.51.
-//   d = 128  0.517 (1,200 TFLOP/s, 0.71 of the measured bf16 peak): MMAs and barriers alone 0.45
-//
-// The accumulator is rescaled only when a row's maximum has grown by more than
-// kSlack (in powers of two) over the one in use: the softmax is the same for
-// any reference near the maximum, p <= 2^kSlack stays well inside f32 and f16,
-// and a rescale is a round trip of O through TMEM. P is rounded to the input
-// type (8 or 11 bits, as v has); its sum is taken before that, in f32.
+// Weights are taken against the maximum of the blocks before. The block's own
+// maximum is found along the way, and only where it has grown by more than
+// kSlack (in powers of two) is it taken over: O is rescaled, a round trip
+// through TMEM, and the block's weights are computed again from the scores in
+// registers. The softmax is the same for any reference near the maximum. P is
+// rounded to the input type (8 or 11 bits, as v has); its sum is taken before
+// that, in f32.
 //
 // Rows past the block's keys: their scores are replaced by -inf (so p is 0)
 // and their V rows by zeros in shared memory, whatever they hold.
+//
+// What bounds it (one B200, dense, 4,096 x 4,096 rows, 128 x 64 tiles):
+//   d = 64   148 heads, 827 us, 768 TFLOP/s (0.45 of the measured bf16 peak). The softmax warps: 64
+//            exponentials a row and tile at 16 a cycle and SM are 512 cycles, a tile takes about 690
+//            (1.7 GHz under this load); MMAs and barriers alone 540 us. A part of the exponentials on
+//            the FMA pipe (a polynomial): 851 us with one in eight, 894 with two. Two threads per row, or
+//            two groups of softmax warps per CTA: 909, 896. One warp for all MMAs: 868.
+//   d = 128  74 heads, 523 us, 1,215 TFLOP/s (0.72): MMAs and barriers alone 456 us
 #include <cmath>
 
 #include "tc_common.cuh"
@@ -42,12 +45,10 @@ namespace {
 
 constexpr int kQ = kAttnQRows, kK = kAttnKRows;
 constexpr int kQPanel = kQ * 128, kKPanel = kK * 128;  // bytes of 64 columns of a Q / K / V tile
-constexpr float kSlack = 8.f;
-// pairs of eight whose exponentials go to the FMA pipe (exp2_poly) instead of
-// the special-function unit, which gives 16 a cycle and SM: at d = 64, 4096^2
-// rows x 148 heads, 0 / 1 / 2 / 3 of eight took 910 / 903 / 893 / 960 us
-constexpr int kPolyOfEight = 2;
-
+// how far (in powers of two) a row's maximum may grow past the one in use: a
+// weight up to 2^24 is as exact in bf16 and f32 as one up to 1; f16 ends at 65,504
+template <bool kF16>
+constexpr float kSlack = kF16 ? 8.f : 24.f;
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
@@ -60,6 +61,8 @@ struct AttnParams {
     int n_qb;   // tile t: query block t % n_qb, heads from (t / n_qb) * pack
     int chunk, chunks;  // CTAs that share a tile's list, and list entries of each
     float c;    // scale * log2(e)
+    const void* q;
+    int64_t q_stride;
     void* out;
     int64_t out_stride;
     int tile_rows;   // most rows of a tile
@@ -74,15 +77,19 @@ struct AttnParams {
 template <int D>
 struct Cfg {
     static constexpr int kPanels = D / 64;
-    static constexpr int kBufs = D == 64 ? 3 : 2;  // blocks whose scores are computed ahead of the softmax
+    // Q as a TMEM operand where the accumulator leaves the columns: Q K^T then reads only K from shared
+    // memory (d = 64: 827 against 850 us); else in shared memory
+    static constexpr bool kQTmem = D == 64;
+    static constexpr int kBufs = 2;            // blocks whose scores are computed ahead of the softmax
     static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;
     static constexpr int kThreads = 128 + 64;
     static constexpr int kTmemCols = 256;
-    static constexpr int kOCol = 64 * kBufs;  // S buffers | O
-    static_assert(kOCol + D == kTmemCols, "TMEM");
-    // q_full | k_full, k_empty [kKS] | v_full, v_empty [kVS] | s_full, p_full, o_done [kBufs] | drained
-    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 3 * kBufs + 1;
-    static constexpr size_t kTiles = (size_t)kPanels * kQPanel + (size_t)(kKS + kVS) * kPanels * kKPanel;
+    static constexpr int kOCol = 64 * kBufs, kQCol = kOCol + D;  // S buffers | O | Q
+    static_assert(kQCol + (kQTmem ? D / 2 : 0) <= kTmemCols, "TMEM");
+    // q_full | k_full, k_empty [kKS] | v_full, v_empty [kVS] | s_full, p_full, o_done [kBufs] | drained [2]
+    static constexpr int kBars = 1 + 2 * kKS + 2 * kVS + 3 * kBufs + 2;
+    static constexpr int kQBytes = kQTmem ? 0 : kPanels * kQPanel;
+    static constexpr size_t kTiles = kQBytes + (size_t)(kKS + kVS) * kPanels * kKPanel;
     static constexpr size_t smem(int list) { return 1024 + kTiles + kBars * 8 + 16 + (size_t)list * 4; }
 };
 
@@ -146,6 +153,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::S3DSP_I8(v, 0),
+        S3DSP_I8(v, 8), S3DSP_I8(v, 16), S3DSP_I8(v, 24), "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::S3DSP_I8(v, 0), "r"(taddr)
                  : "memory");
@@ -203,32 +217,6 @@ __device__ __forceinline__ F2 add2v(F2 a, F2 b) {
     return d;
 }
 __device__ __forceinline__ F2 both(float v) { return F2{v, v}; }
-// 2^x on the FMA and integer pipes, for x <= kSlack: x = n + f with n the
-// nearest whole number (read off the low bits of x + 1.5 * 2^23), a minimax
-// polynomial of 2^f on [-1/2, 1/2] (Remez exchange on the relative error:
-// 7.5e-5 of degree 3, far below bf16's rounding of the weight; 2.7e-6 of degree
-// 4 for f16), and n added to the exponent. x below -126 counts as -126.
-template <bool kF16>
-__device__ __forceinline__ F2 exp2_poly(F2 x) {
-    constexpr float kMagic = 12582912.f;
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const F2 t = add2v(x, both(kMagic));
-    const F2 f = add2v(x, fma2v(add2v(t, both(-kMagic)), both(-1.f), both(0.f)));
-    F2 p;
-    if constexpr (kF16) {
-        p = fma2v(both(0.009570102207362652f), f, both(0.05591785907745361f));
-        p = fma2v(p, f, both(0.240247443318367f));
-        p = fma2v(p, f, both(0.6931217908859253f));
-        p = fma2v(p, f, both(0.9999992847442627f));
-    } else {
-        p = fma2v(both(0.0551716685295105f), f, both(0.2426111251115799f));
-        p = fma2v(p, f, both(0.6932609677314758f));
-        p = fma2v(p, f, both(0.9999280571937561f));
-    }
-    return F2{__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-              __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23))};
-}
 // (lo, hi) as two 16-bit floats of one register
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -249,7 +237,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t* sm = raw + (base - smem_u32(raw));
-    const uint32_t sQ = base, sK = sQ + C::kPanels * kQPanel, sV = sK + C::kKS * C::kPanels * kKPanel;
+    const uint32_t sQ = base, sK = sQ + C::kQBytes, sV = sK + C::kKS * C::kPanels * kKPanel;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::kTiles);
     const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, k_empty = k_full + 8 * C::kKS,
                    v_full = k_empty + 8 * C::kKS, v_empty = v_full + 8 * C::kVS, s_full = v_empty + 8 * C::kVS,
@@ -261,19 +249,20 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     int* list = reinterpret_cast<int*>(bars + C::kBars) + 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kProdWarp = 4, kMmaWarp = 5;
+    constexpr int kKeyWarp = 4, kValueWarp = 5;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
+        mbar_init(q_full, C::kQTmem ? 4 : 1);
         for (int s = 0; s < C::kKS; ++s) mbar_init(k_full + 8 * s, 1), mbar_init(k_empty + 8 * s, 1);
         for (int s = 0; s < C::kVS; ++s) mbar_init(v_full + 8 * s, 1), mbar_init(v_empty + 8 * s, 1);
         for (int s = 0; s < B; ++s)
             mbar_init(s_full + 8 * s, 1), mbar_init(p_full + 8 * s, 4), mbar_init(o_done + 8 * s, 1);
         mbar_init(drained, 1);
+        mbar_init(drained + 8, 1);
         *abort_flag = 0;
         *drain_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == kValueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                      "r"((uint32_t)C::kTmemCols)
                      : "memory");
@@ -310,93 +299,112 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     const uint32_t tmem = *tmem_holder;
     const int n = split ? max(0, min(p.chunk, *n_listed - first)) : *n_listed;
     auto block_of = [&](int j) { return p.sel ? list[first + j] : first + j; };
-    auto rows_of = [&](int blk) { return min(kK, k_rows - blk * kK); };
+    const int last_block = nkb - 1, last_rows = k_rows - last_block * kK;  // the sequence's last block may be short
 
-    if (warp == kProdWarp) {
-        // ================= TMA producer =================
+    // after a wait gave up: the copies and MMAs that this thread has issued land
+    // before shared memory and TMEM are given back
+    auto drain = [&](uint32_t full, int ring, int loaded, bool q) {
+        if (q) mbar_wait(q_full, 0, drain_flag, p.status);
+        for (int j = max(0, loaded - ring); j < loaded; ++j)
+            mbar_wait(full + 8 * (j % ring), (j / ring) & 1, drain_flag, p.status);
+        mma_commit(drained + 8 * (warp & 1));
+        mbar_wait(drained + 8 * (warp & 1), 0, drain_flag, p.status);
+    };
+    constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
+    constexpr uint32_t kFmt = kF16 ? 0u : 1u;
+    auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
+    if (warp == kKeyWarp) {
+        // ================= K tiles, and S = Q K^T =================
         if (n > 0 && elect_one()) {
-            constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
+            constexpr uint32_t kIdesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kK >> 3) << 17) | ((kQ >> 4) << 24);
             const int kc = (h / p.per_kv) * D;
-            mbar_arrive_tx(q_full, C::kPanels * kQPanel);
-            for (int i = 0; i < C::kPanels; ++i) tma_load_3d(sQ + i * kQPanel, &qmap, 64 * i, h, q_row0, q_full);
-            int issued_k = 0, issued_v = 0;
-            bool ok = true;
-            Cursor<C::kKS> ks;
-            Cursor<C::kVS> vs;
-            for (int j = 0; j < n && ok; ++j, ks.next(), vs.next()) {
-                const int y = k_row0 + block_of(j) * kK;
-                ok = mbar_wait(k_empty + 8 * ks.slot, ks.parity ^ 1u, abort_flag, p.status);
-                if (!ok) break;
-                mbar_arrive_tx(k_full + 8 * ks.slot, kTileBytes);
+            int loaded = 0;
+            Cursor<C::kKS> ls;  // the next tile's place
+            auto load = [&]() {
+                const int y = k_row0 + block_of(loaded) * kK;
+                mbar_arrive_tx(k_full + 8 * ls.slot, kTileBytes);
                 for (int i = 0; i < C::kPanels; ++i)
-                    tma_load_2d(sK + ks.slot * kTileBytes + i * kKPanel, &kmap, kc + 64 * i, y, k_full + 8 * ks.slot);
-                ++issued_k;
-                ok = mbar_wait(v_empty + 8 * vs.slot, vs.parity ^ 1u, abort_flag, p.status);
+                    tma_load_2d(sK + ls.slot * kTileBytes + i * kKPanel, &kmap, kc + 64 * i, y, k_full + 8 * ls.slot);
+                ls.next();
+                ++loaded;
+            };
+            if constexpr (!C::kQTmem) {
+                mbar_arrive_tx(q_full, C::kPanels * kQPanel);
+                for (int i = 0; i < C::kPanels; ++i) tma_load_3d(sQ + i * kQPanel, &qmap, 64 * i, h, q_row0, q_full);
+            }
+            while (loaded < min(n, C::kKS)) load();
+            bool ok = wait(q_full, 0);
+            tc_fence_after();
+            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK);
+            Cursor<C::kKS> ks, es;  // the tile, and the oldest one whose place may be free
+            Cursor<B> sb, ob;        // the score buffer, and the product that last read it
+            for (int j = 0; j < n && ok; ++j, ks.next(), sb.next()) {
+                if (j > 0 && loaded < n) {
+                    // the tile before this one has been read: another takes its place
+                    ok = wait(k_empty + 8 * es.slot, es.parity);
+                    es.next();
+                    if (ok) load();
+                }
+                if (j >= B) {
+                    ok = ok && wait(o_done + 8 * ob.slot, ob.parity);
+                    ob.next();
+                }
+                ok = ok && wait(k_full + 8 * ks.slot, ks.parity);
                 if (!ok) break;
-                mbar_arrive_tx(v_full + 8 * vs.slot, kTileBytes);
-                for (int i = 0; i < C::kPanels; ++i)
-                    tma_load_2d(sV + vs.slot * kTileBytes + i * kKPanel, &vmap, kc + 64 * i, y, v_full + 8 * vs.slot);
-                ++issued_v;
-            }
-            if (!ok) {
-                // this CTA's copies land before its shared memory is given back
-                mbar_wait(q_full, 0, drain_flag, p.status);
-                for (int j = max(0, issued_k - C::kKS); j < issued_k; ++j)
-                    mbar_wait(k_full + 8 * (j % C::kKS), (j / C::kKS) & 1, drain_flag, p.status);
-                for (int j = max(0, issued_v - C::kVS); j < issued_v; ++j)
-                    mbar_wait(v_full + 8 * (j % C::kVS), (j / C::kVS) & 1, drain_flag, p.status);
-            }
-        }
-        __syncwarp();
-    } else if (warp == kMmaWarp) {
-        // ================= MMA issuer =================
-        if (n > 0 && elect_one()) {
-            constexpr uint32_t kFmt = kF16 ? 0u : 1u;
-            constexpr uint32_t kIdescQK = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((kK >> 3) << 17) | ((kQ >> 4) << 24);
-            constexpr uint32_t kIdescPV = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) |
-                                          ((kQ >> 4) << 24);
-            constexpr uint32_t kTileBytes = C::kPanels * kKPanel;
-            auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status); };
-            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dv = mn_desc(sV);
-            Cursor<C::kKS> ks;  // the next K tile, score buffer
-            Cursor<B> sb;
-            auto qk = [&]() {
-                if (!wait(k_full + 8 * ks.slot, ks.parity)) return false;
                 tc_fence_after();
                 const uint64_t dkt = dk + ((ks.slot * kTileBytes) >> 4);
 #pragma unroll
-                for (int x = 0; x < D / 16; ++x)
-                    mma_bf16(tmem + 64 * sb.slot, dq + (((x / 4) * kQPanel + (x % 4) * 32) >> 4),
-                             dkt + (((x / 4) * kKPanel + (x % 4) * 32) >> 4), kIdescQK, x > 0);
+                for (int x = 0; x < D / 16; ++x) {
+                    const uint64_t b = dkt + (((x / 4) * kKPanel + (x % 4) * 32) >> 4);
+                    if constexpr (C::kQTmem)
+                        mma_ts(tmem + 64 * sb.slot, tmem + C::kQCol + 8 * x, b, kIdesc, x > 0);
+                    else
+                        mma_bf16(tmem + 64 * sb.slot, dq + (((x / 4) * kQPanel + (x % 4) * 32) >> 4), b, kIdesc, x > 0);
+                }
                 mma_commit(s_full + 8 * sb.slot);
                 mma_commit(k_empty + 8 * ks.slot);
-                ks.next();
-                sb.next();
-                return true;
+            }
+            if (!ok) drain(k_full, C::kKS, loaded, !C::kQTmem);
+        }
+        __syncwarp();
+    } else if (warp == kValueWarp) {
+        // ================= V tiles, and O += P V =================
+        if (n > 0 && elect_one()) {
+            constexpr uint32_t kIdesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((D >> 3) << 17) | ((kQ >> 4) << 24);
+            const int kc = (h / p.per_kv) * D;
+            int loaded = 0;
+            Cursor<C::kVS> ls;
+            auto load = [&]() {
+                const int y = k_row0 + block_of(loaded) * kK;
+                mbar_arrive_tx(v_full + 8 * ls.slot, kTileBytes);
+                for (int i = 0; i < C::kPanels; ++i)
+                    tma_load_2d(sV + ls.slot * kTileBytes + i * kKPanel, &vmap, kc + 64 * i, y, v_full + 8 * ls.slot);
+                ls.next();
+                ++loaded;
             };
-            bool ok = wait(q_full, 0);
-            for (int j = 0; j < min(n, B) && ok; ++j) ok = qk();
-            Cursor<C::kVS> vs;
+            while (loaded < min(n, C::kVS)) load();
+            const uint64_t dv = mn_desc(sV);
+            bool ok = true;
+            Cursor<C::kVS> vs, es;
             Cursor<B> pb;
             for (int j = 0; j < n && ok; ++j, vs.next(), pb.next()) {
-                ok = wait(v_full + 8 * vs.slot, vs.parity) && wait(p_full + 8 * pb.slot, pb.parity);
+                if (j > 0 && loaded < n) {
+                    ok = wait(v_empty + 8 * es.slot, es.parity);
+                    es.next();
+                    if (ok) load();
+                }
+                ok = ok && wait(v_full + 8 * vs.slot, vs.parity) && wait(p_full + 8 * pb.slot, pb.parity);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t dvt = dv + ((vs.slot * kTileBytes) >> 4);
 #pragma unroll
                 for (int x = 0; x < kK / 16; ++x)
-                    mma_ts(tmem + C::kOCol, tmem + 64 * pb.slot + 8 * x, dvt + ((x * 2048) >> 4), kIdescPV,
+                    mma_ts(tmem + C::kOCol, tmem + 64 * pb.slot + 8 * x, dvt + ((x * 2048) >> 4), kIdesc,
                            (j > 0 || x > 0) ? 1u : 0u);
                 mma_commit(o_done + 8 * pb.slot);
                 mma_commit(v_empty + 8 * vs.slot);
-                // this buffer's next scores, once its weights have been read
-                if (j + B < n) ok = wait(o_done + 8 * pb.slot, pb.parity) && qk();
             }
-            if (!ok) {
-                // the MMAs issued so far end before their operands are given back
-                mma_commit(drained);
-                mbar_wait(drained, 0, drain_flag, p.status);
-            }
+            if (!ok) drain(v_full, C::kVS, loaded, false);
         }
         __syncwarp();
     } else {
@@ -411,11 +419,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         };
         Cursor<B> sb, ob;  // the block's buffer, and that of the product before it
         // V rows of block j that are not the sequence's: zeros (p is 0 there, and 0 * NaN is not)
-        auto clear_tail = [&](int j, int rows) {
+        auto clear_tail = [&](int j) {
             const int t = j % C::kVS;
             if (!wait(v_full + 8 * t, (j / C::kVS) & 1)) return false;
             for (int x = 0; x < C::kPanels; ++x)
-                for (int a = rows * 128 + row * 16; a < kKPanel; a += kQ * 16)
+                for (int a = last_rows * 128 + row * 16; a < kKPanel; a += kQ * 16)
                     *reinterpret_cast<uint4*>(sm + (sV - base) + (t * C::kPanels + x) * kKPanel + a) = make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             return true;
@@ -427,6 +435,26 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             ob = sb;
             sb.next();
         };
+        if (C::kQTmem && n > 0) {
+            // this row of Q into TMEM, two values a column (rows that are not there are never looked at)
+            if (live) {
+                uint32_t w[32];
+                const int64_t q_row = q_row0 + row / p.pack;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_row * p.q_stride +
+                                                                  (int64_t)(h + row % p.pack) * D);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const uint4 v = row < q_rows ? __ldg(src + x) : make_uint4(0, 0, 0, 0);
+                    w[4 * x] = v.x, w[4 * x + 1] = v.y, w[4 * x + 2] = v.z, w[4 * x + 3] = v.w;
+                }
+                tmem_st32(t0 + C::kQCol, w);
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        bool short_block = last_rows < kK && n > 0 && block_of(0) == last_block;
         for (int j = 0; live && j < n; ++j) {
             const uint32_t ts = t0 + 64 * sb.slot;
             ok = wait(s_full + 8 * sb.slot, sb.parity);
@@ -438,23 +466,49 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             tmem_wait_ld();
             tmem_settle(s[0]);
             tmem_settle(s[1]);
-            const int rows = rows_of(block_of(j));
-            if (rows < kK) {
+            if (short_block) {
 #pragma unroll
                 for (int x = 0; x < kK; ++x)
-                    if (x >= rows) s[x / 32][x % 32] = 0xff800000u;  // -inf
-                ok = clear_tail(j, rows);
+                    if (x >= last_rows) s[x / 32][x % 32] = 0xff800000u;  // -inf
+                ok = clear_tail(j);
                 if (!ok) break;
             }
-            // the running maximum, and a rescale of O and l where it has grown
-            float mx[4] = {m, m, m, m};
+            short_block = last_rows < kK && j + 1 < n && block_of(j + 1) == last_block;  // of the next step
+            // The weights against the maximum so far, into the scores' first columns, and their sum; the
+            // block's own maximum is found along the way. Only where that has grown by more than kSlack
+            // does the row take it over: O and l are rescaled and the weights computed again (the scores
+            // are still in registers).
+            if (j == 0) {
+                float mx[4] = {m, m, m, m};
 #pragma unroll
-            for (int x = 0; x < kK; x += 2)
-                mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x / 32][x % 32]), __uint_as_float(s[x / 32][x % 32 + 1]));
-            const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-            // a NaN maximum always counts as grown, and stays
-            const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
-            if (__any_sync(0xffffffffu, grown)) {
+                for (int x = 0; x < kK; x += 2)
+                    mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x / 32][x % 32]), __uint_as_float(s[x / 32][x % 32 + 1]));
+                m = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            }
+            F2 sum[2];
+            for (int attempt = 0;; ++attempt) {
+                // (an infinite maximum makes its row NaN, as inf - inf does)
+                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
+                float mx[2] = {m, m};
+                sum[0] = sum[1] = both(0.f);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const F2 sc = {__uint_as_float(s[half][2 * x]), __uint_as_float(s[half][2 * x + 1])};
+                        mx[x & 1] = max3(mx[x & 1], sc.x, sc.y);
+                        F2 v = fma2v(sc, both(p.c), bias);
+                        v = F2{exp2_hw(v.x), exp2_hw(v.y)};
+                        sum[x & 1] = add2v(sum[x & 1], v);
+                        w[x] = pack2<kF16>(v.x, v.y);
+                    }
+                    tmem_st16(ts + 16 * half, w);
+                }
+                const float mt = max3(mx[0], mx[1], mx[1]);
+                // a NaN maximum counts as grown, and stays
+                const bool grown = !((mt - m) * p.c <= kSlack<kF16>) && !(mt == -INFINITY);
+                if (attempt > 0 || !__any_sync(0xffffffffu, grown)) break;
                 const float to = grown ? mt : m;
                 const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
                 if (j > 0) {
@@ -473,25 +527,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
                 l *= alpha;
                 m = to;
             }
-            // the weights, into the scores' first columns, and their sum
-            // (an infinite maximum makes its row NaN, as inf - inf does)
-            const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
-            F2 sum[2] = {both(0.f), both(0.f)};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t w[16];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    F2 v = fma2v(F2{__uint_as_float(s[half][2 * x]), __uint_as_float(s[half][2 * x + 1])}, both(p.c), bias);
-                    if ((x & 7) < kPolyOfEight)
-                        v = exp2_poly<kF16>(v);
-                    else
-                        v = F2{exp2_hw(v.x), exp2_hw(v.y)};
-                    sum[x & 1] = add2v(sum[x & 1], v);
-                    w[x] = pack2<kF16>(v.x, v.y);
-                }
-                tmem_st16(ts + 16 * half, w);
-            }
+            if (!ok) break;
             const F2 total = add2v(sum[0], sum[1]);
             l += total.x + total.y;
             tmem_wait_st();
@@ -499,8 +535,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         }
         for (int j = 0; !live && j < n && ok; ++j) {
             ok = wait(s_full + 8 * sb.slot, sb.parity);
-            const int rows = rows_of(block_of(j));
-            if (ok && rows < kK) ok = clear_tail(j, rows);
+            if (ok && last_rows < kK && block_of(j) == last_block) ok = clear_tail(j);
             if (ok) hand_over();
         }
         // the last product (they complete in order). A wait tells two neighbouring phases of its
@@ -508,8 +543,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         if (ok && n > 0) ok = wait(o_done + 8 * ((n - 1) % B), ((n - 1) / B) & 1);
         tc_fence_after();
         if (ok && live) {
-            // nothing listed, or every score -inf (exp2_poly gives those a weight of 2^-126, not 0)
-            const bool none = m == -INFINITY || l == 0.f;
+            const bool none = l == 0.f;  // nothing listed, or every score -inf
             const float inv = none ? 0.f : 1.f / l;
             const int64_t q_row = q_row0 + row / p.pack;
             const int head = h + row % p.pack;
@@ -550,7 +584,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kValueWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::kTmemCols));
     }
@@ -738,6 +772,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.chunks = (int)chunks;
     p.tile_rows = plan->max_q_rows * pack;
     p.c = scale * 1.4426950408889634f;
+    p.q = q;
+    p.q_stride = q_stride;
     p.out = out;
     p.out_stride = out_stride;
     p.status = ctx->d_status;
