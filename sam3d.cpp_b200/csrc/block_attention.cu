@@ -119,6 +119,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "l"((unsigned long long)map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)map) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -268,22 +271,39 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (lane == 0) {
+        if (warp == kKeyWarp) prefetch_map(&kmap);
+        if (warp == kValueWarp) prefetch_map(&vmap);
+    }
     pdl_wait();
     const bool split = p.chunks > 1;
     const int tile = split ? (int)blockIdx.x / p.chunks : (int)blockIdx.x;
     const int first = split ? (int)blockIdx.x % p.chunks * p.chunk : 0;
     const int bq = tile % p.n_qb, h = tile / p.n_qb * p.pack;
-    const int4 qb = p.q_blocks[bq];
+    // the list's first entries and the block's table entry are read together
+    const int32_t* sel = p.sel ? p.sel + ((int64_t)bq * p.heads + h) * p.top : nullptr;
+    int e = -1;
+    if (warp == 0 && lane < p.top) e = __ldg(sel + lane);
+    const int4 qb = __ldg(p.q_blocks + bq);
     const int q_row0 = qb.x, q_rows = (qb.y & kAttnRowsMask) * p.pack, k_row0 = qb.z, k_rows = qb.w;
     const int nkb = (k_rows + kK - 1) / kK;
+    // the softmax threads' rows of Q, on their way while the list is made
+    const bool has_row = threadIdx.x < q_rows;
+    uint4 q_row[C::kQTmem ? D / 8 : 1];
+    if (C::kQTmem && warp < 4) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const uint16_t*>(p.q) + (q_row0 + (has_row ? (int)threadIdx.x / p.pack : 0)) * p.q_stride +
+            (int64_t)(h + (has_row ? (int)threadIdx.x % p.pack : 0)) * D);
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) q_row[x] = has_row ? __ldg(src + x) : make_uint4(0, 0, 0, 0);
+    }
     if (warp == 0) {
         // the listed blocks that exist, in list order
         int n = nkb;
-        if (p.sel) {
-            const int32_t* row = p.sel + ((int64_t)bq * p.heads + h) * p.top;
+        if (sel) {
             n = 0;
             for (int i0 = 0; i0 < p.top; i0 += 32) {
-                const int e = i0 + lane < p.top ? __ldg(row + i0 + lane) : -1;
+                if (i0 > 0) e = i0 + lane < p.top ? __ldg(sel + i0 + lane) : -1;
                 if (e >= nkb) atomicOr(p.status, kErrRowRange);
                 const unsigned m = __ballot_sync(0xffffffffu, e >= 0 && e < nkb);
                 if (e >= 0 && e < nkb) list[n + __popc(m & ((1u << lane) - 1u))] = e;
@@ -435,18 +455,13 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
             ob = sb;
             sb.next();
         };
-        if (C::kQTmem && n > 0) {
+        if constexpr (C::kQTmem) if (n > 0) {
             // this row of Q into TMEM, two values a column (rows that are not there are never looked at)
             if (live) {
                 uint32_t w[32];
-                const int64_t q_row = q_row0 + row / p.pack;
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_row * p.q_stride +
-                                                                  (int64_t)(h + row % p.pack) * D);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const uint4 v = row < q_rows ? __ldg(src + x) : make_uint4(0, 0, 0, 0);
-                    w[4 * x] = v.x, w[4 * x + 1] = v.y, w[4 * x + 2] = v.z, w[4 * x + 3] = v.w;
-                }
+                for (int x = 0; x < 8; ++x)
+                    w[4 * x] = q_row[x].x, w[4 * x + 1] = q_row[x].y, w[4 * x + 2] = q_row[x].z, w[4 * x + 3] = q_row[x].w;
                 tmem_st32(t0 + C::kQCol, w);
                 tmem_wait_st();
             }
@@ -545,12 +560,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         if (ok && live) {
             const bool none = l == 0.f;  // nothing listed, or every score -inf
             const float inv = none ? 0.f : 1.f / l;
-            const int64_t q_row = q_row0 + row / p.pack;
+            const int64_t out_row = q_row0 + row / p.pack;
             const int head = h + row % p.pack;
             const int64_t part = (int64_t)blockIdx.x * p.tile_rows + row;
             if (split && row < q_rows) p.part_ml[part] = make_float2(m, l);
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + q_row * p.out_stride + (int64_t)head * D;
-#pragma unroll 1
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D;
+#pragma unroll
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t o[32];
                 if (n > 0) {
