@@ -265,12 +265,6 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
         *drain_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kValueWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                     "r"((uint32_t)C::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     if (lane == 0) {
         if (warp == kKeyWarp) prefetch_map(&kmap);
         if (warp == kValueWarp) prefetch_map(&vmap);
@@ -287,6 +281,17 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     const int4 qb = __ldg(p.q_blocks + bq);
     const int q_row0 = qb.x, q_rows = (qb.y & kAttnRowsMask) * p.pack, k_row0 = qb.z, k_rows = qb.w;
     const int nkb = (k_rows + kK - 1) / kK;
+    if (split && !sel && first >= nkb) {
+        // a chunk past a short list: nothing to add
+        if ((int)threadIdx.x < q_rows) p.part_ml[(int64_t)blockIdx.x * p.tile_rows + threadIdx.x] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    if (warp == kValueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"((uint32_t)C::kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     // the softmax threads' rows of Q, on their way while the list is made
     const bool has_row = threadIdx.x < q_rows;
     uint4 q_row[C::kQTmem ? D / 8 : 1];
@@ -605,53 +610,76 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
     }
 }
 
-// Joins the chunks of a tile's rows: sums weighed by 2^(c (m_z - max m)).
-// One warp per row, D / 32 columns per lane; a chunk without blocks has
-// m = -inf and is not read.
+// Joins the chunks of a tile's rows: sums weighed by 2^(c (m_z - max m)). One
+// CTA per row: warp w adds chunks w, w + 8, ..., D / 32 columns per lane, and the
+// warps' sums are added in order. A chunk without blocks has m = -inf and is
+// not read.
+constexpr int kJoinWarps = 8;
 template <int D, bool kF16>
-__global__ void __launch_bounds__(256) join_chunks_kernel(const AttnParams p, int64_t items) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const AttnParams p) {
+    __shared__ float sums[kJoinWarps][D + 1];
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= items) return;
-    const int tile = (int)(item / p.tile_rows), row = (int)(item % p.tile_rows);
+    constexpr int kC = D / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile = blockIdx.x / p.tile_rows, row = blockIdx.x % p.tile_rows;
+    const int64_t step = p.tile_rows, at = (int64_t)tile * p.chunks * step + row;
+    // every warp has all chunks' (m, l), chunk 32 i + lane in slot i
+    float2 ml[kMaxChunks / 32];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / 32; ++i) {
+        const int z = 32 * i + lane;
+        ml[i] = z < p.chunks ? p.part_ml[z * step + at] : make_float2(-INFINITY, 0.f);
+    }
     const int4 qb = p.q_blocks[tile % p.n_qb];
     if (row >= (qb.y & kAttnRowsMask) * p.pack) return;
-    const int64_t q_row = qb.x + row / p.pack, step = p.tile_rows;
-    const int64_t at = (int64_t)tile * p.chunks * step + row;
-    const int head = tile / p.n_qb * p.pack + row % p.pack;
-    float top = -INFINITY;
-    for (int z = lane; z < p.chunks; z += 32) {
-        const float m = p.part_ml[z * step + at].x;
-        top = max3(top, m, m);
-    }
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / 32; ++i) top = max3(top, ml[i].x, ml[i].x);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) {
         const float m = __shfl_xor_sync(0xffffffffu, top, x);
         top = max3(top, m, m);
     }
-    float acc[D / 32], l = 0.f;
+    float acc[kC], l = 0.f;
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
+    for (int x = 0; x < kC; ++x) acc[x] = 0.f;
     if (!(top == -INFINITY)) {
-#pragma unroll 4
-        for (int z = 0; z < p.chunks; ++z) {
-            const float2 ml = p.part_ml[z * step + at];
-            if (ml.x == -INFINITY) continue;
-            const float w = exp2_hw((ml.x - top) * p.c);
-            l = fmaf(w, ml.y, l);
-            const float* o = p.part_o + (z * step + at) * D + lane * (D / 32);
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) acc[x] = fmaf(w, o[x], acc[x]);
+        for (int i = 0; i < kMaxChunks / 32; ++i) {
+            const float wl = ml[i].x == -INFINITY ? 0.f : exp2_hw((ml[i].x - top) * p.c);  // the chunk's weight
+            const unsigned some = __ballot_sync(0xffffffffu, !(ml[i].x == -INFINITY));
+#pragma unroll
+            for (int b = 0; b < 32; b += kJoinWarps) {
+                const int src = b + warp;
+                const float w = __shfl_sync(0xffffffffu, wl, src), lz = __shfl_sync(0xffffffffu, ml[i].y, src);
+                if (!(some >> src & 1u)) continue;
+                l = fmaf(w, lz, l);
+                const float* o = p.part_o + ((32 * i + src) * step + at) * D + lane * kC;
+#pragma unroll
+                for (int x = 0; x < kC; ++x) acc[x] = fmaf(w, __ldg(o + x), acc[x]);
+            }
         }
     }
-    const bool none = top == -INFINITY || l == 0.f;
-    const float inv = none ? 0.f : 1.f / l;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + q_row * p.out_stride + (int64_t)head * D +
-                                                lane * (D / 32));
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) dst[x] = none ? 0u : pack2<kF16>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+    for (int x = 0; x < kC; ++x) sums[warp][lane * kC + x] = acc[x];
+    if (lane == 0) sums[warp][D] = l;
+    __syncthreads();
+    if (threadIdx.x >= D / 2) return;
+    float a0 = 0.f, a1 = 0.f;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        a0 += sums[w][2 * threadIdx.x];
+        a1 += sums[w][2 * threadIdx.x + 1];
+        l += sums[w][D];
+    }
+    const bool none = l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    const int64_t out_row = qb.x + row / p.pack;
+    const int head = tile / p.n_qb * p.pack + row % p.pack;
+    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D)[threadIdx.x] =
+        none ? 0u : pack2<kF16>(a0 * inv, a1 * inv);
 }
 
 // [rows][cols] 16-bit rows, tiles of box_rows x 64 columns with the 128-byte swizzle
@@ -699,8 +727,8 @@ cudaError_t launch(s3dsp_context* ctx, dim3 grid, const CUtensorMap& q, const CU
     e = launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
                    ctx->stream, q, k, v, p);
     if (e != cudaSuccess || p.chunks == 1) return e;
-    const int64_t items = (int64_t)grid.x / p.chunks * p.tile_rows;
-    return launch_pdl(join_chunks_kernel<D, kF16>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, ctx->stream, p, items);
+    return launch_pdl(join_chunks_kernel<D, kF16>, dim3(grid.x / p.chunks * p.tile_rows), dim3(32 * kJoinWarps), 0,
+                      ctx->stream, p);
 }
 
 }  // namespace
@@ -756,7 +784,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // lengths differ. A chunk has at least kMinChunk blocks, and the split has
     // to save kMinSaved: a block takes a CTA about 0.9 us, the joining kernel
     // and its traffic about 8. (8 rows over 92k keys, 4 key heads: 527 us
-    // without, 68 with. Sharing only the tiles of a last, half empty wave was
+    // without, @@ with. Sharing only the tiles of a last, half empty wave was
     // measured too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on
     // an SM runs 1.2x as fast as one of two.)
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
@@ -764,7 +792,9 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
     int64_t chunk = longest, chunks = 1;
     if (tiles <= slots / 2) {
-        chunk = ((d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * (heads / pack) + slots - 1) / slots;
+        // sum over the lists of ceil(length / chunk) <= (their sum) / chunk + their number
+        const int64_t lists = slots / (heads / pack) - plan->n_qb;
+        chunk = ((d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) + lists - 1) / (lists > 0 ? lists : 1);
         if (chunk < kMinChunk) chunk = kMinChunk;
         if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
         if (longest - chunk >= kMinSaved) chunks = (longest + chunk - 1) / chunk;
