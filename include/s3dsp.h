@@ -429,7 +429,9 @@ S3DSP_API s3d_status s3dsp_qk_norm_rope(s3dsp_context *ctx, const void *q, int64
  * S3DSP_ATTN_Q_ROWS rows and key blocks of S3DSP_ATTN_K_ROWS, counted from
  * its own first row, the last ones shorter. Made from host memory on the
  * context's stream (not inside a stream capture; calls that use the plan may
- * be captured). Freed by s3dsp_attn_plan_free. */
+ * be captured). Other contexts of the device may use the plan once that
+ * stream has passed the call. Freed by s3dsp_attn_plan_free, in order of the
+ * stream of the context it is given. */
 S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context *ctx, const int64_t *h_q_offsets,
                                             const int64_t *h_k_offsets, int64_t n_seq, s3dsp_attn_plan **out,
                                             char *error, uint64_t error_capacity);

@@ -83,6 +83,11 @@ struct Cfg {
     static constexpr int kBufs = 2;            // blocks whose scores are computed ahead of the softmax
     static constexpr int kKS = D == 64 ? 4 : 2, kVS = kKS;
     static constexpr int kThreads = 128 + 64;
+    // d = 128 takes registers as for 8 warps (128 each). With the 168 that six warps allow, two CTAs of
+    // six fit on an SM only where they put their pairs of warps on different schedulers, which they do
+    // not always after CTAs of different lengths (8 single rows: 64 against 58 us). d = 64 takes the
+    // registers all the same: 827 against 843 us dense, 521 against 536 sparse.
+    static constexpr int kRegThreads = D == 64 ? kThreads : 256;
     static constexpr int kTmemCols = 256;
     static constexpr int kOCol = 64 * kBufs, kQCol = kOCol + D;  // S buffers | O | Q
     static_assert(kQCol + (kQTmem ? D / 2 : 0) <= kTmemCols, "TMEM");
@@ -232,7 +237,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 template <int D, bool kF16>
-__global__ void __launch_bounds__(Cfg<D>::kThreads, 2)
+__global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
     block_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                            const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
     using C = Cfg<D>;
@@ -766,6 +771,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     if (plan->n_qb == 0) return S3D_OK;
     if (!q || !out || (plan->n_k > 0 && (!k || !v)))
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "NULL argument");
+    if (out == q || out == k || out == v)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "out must not overlap q, k or v");
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointers need 16-byte alignment");
     S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
@@ -784,7 +791,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // lengths differ. A chunk has at least kMinChunk blocks, and the split has
     // to save kMinSaved: a block takes a CTA about 0.9 us, the joining kernel
     // and its traffic about 8. (8 rows over 92k keys, 4 key heads: 527 us
-    // without, @@ with. Sharing only the tiles of a last, half empty wave was
+    // without, 58 with. Sharing only the tiles of a last, half empty wave was
     // measured too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on
     // an SM runs 1.2x as fast as one of two.)
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;

@@ -586,6 +586,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "keep_local needs a plan whose keys are the query rows");
     if (plan->n_qb == 0) return S3D_OK;
     if (!q || !d_sel || (plan->n_k > 0 && !k)) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "NULL argument");
+    if ((int64_t)plan->n_qb * heads > 0x7fffffff)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "too many query blocks times heads");
     const size_t es = dtype_size(dtype);
     if (((uintptr_t)q | (uintptr_t)k) & (es - 1))
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointer not aligned to its type");

@@ -7,7 +7,8 @@ sparse half around a dense transformer torso:
   input_blocks.0  res_block 128 -> 128, fine map                      (:290-291)
   input_blocks.1  2x mean-pool to the nc coarse voxels, res_block
                   128 -> 1024 on the coarse map, Linear skip          (:294-296)
-  -- APE + transformer blocks on the coarse rows (dense; the caller's) --
+  -- APE + transformer blocks on the coarse rows (the caller's; CoarseAttention
+     is the attention half of such a block on this library) --
   out_blocks.0    concat(h, skip1) 2048 coarse -> nearest upsample ->
                   res_block 2048 -> 128 on the fine map, Linear skip (:463-495)
   out_blocks.1    concat(h, skip0) 256 fine -> res_block 256 -> 128,
@@ -187,3 +188,84 @@ class SlatSparse:
         skip0, skip1 = self.encode(tb, x, mods)
         h = skip1 if mid is None else mid(skip1)
         return self.decode(tb, h, skip0, skip1, mods)
+
+
+class CoarseAttention:
+    """A self-attention layer on the coarse rows, for `forward`'s mid:
+
+        h + out( attention( R(pos) norm(q), R(pos) norm(k), v ) ),  q, k, v = Linears of LayerNorm(h)
+
+    in BF16 with f32 rows h in and out: the per-head norms and the rotation by
+    the voxel position in one pass (s3dsp_qk_norm_rope; a third of a head's
+    pairs for each of x, y, z), attention over every coarse row of the row's
+    object, or with `top` > 0 over the `top` blocks of 64 rows that
+    s3dsp_block_select picks for each 128 query rows and head (the block of the
+    rows themselves among them). The objects of a batch are its sequences."""
+
+    def __init__(self, s3dsp, ctx, params: dict, heads: int, device, top: int = 0, theta: float = 10000.0):
+        import torch
+        self.s, self.ctx, self.torch, self.dev = s3dsp, ctx, torch, device
+        self.c, self.heads, self.top, self.theta = params["out"]["w"].shape[0], heads, top, theta
+        self.pairs = [self.c // heads // 6] * 3
+
+        def dev(a):
+            return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).to(device)
+
+        def lin(d):
+            cout, cin = d["w"].shape
+            dst = torch.empty(s3dsp.Context.packed_bytes(s3dsp.PREC_BF16, 1, cin, cout), dtype=torch.uint8,
+                              device=device)
+            ctx.weights_pack(torch.from_numpy(np.ascontiguousarray(d["w"], dtype=np.float32)), s3dsp.LAYOUT_LINEAR, 1,
+                             cin, cout, s3dsp.PREC_BF16, dst)
+            return dst, dev(d["b"]), cout
+
+        self.q, self.kv, self.out = (lin(params[k]) for k in ("q", "kv", "out"))
+        self.q_gamma, self.k_gamma = dev(params["q_gamma"]), dev(params["k_gamma"])
+
+    def tables(self, tb: SlatTablesDev):
+        """What a batch of objects needs, made once: the coarse coordinates and the attention plan."""
+        t = self.torch
+        coords = t.empty((tb.nc, 4), dtype=t.int32, device=self.dev)
+        self.ctx.slat_tables_export(tb.tables, coarse_coords=coords)
+        rows = t.bincount(coords[:, 0].long()).cpu().numpy()  # coarse rows are sorted by object
+        return coords, self.ctx.attn_plan(np.concatenate([[0], np.cumsum(rows)]))
+
+    def _linear(self, x, wbc, out_dtype, residual=None):
+        w, b, cout = wbc
+        y = self.torch.empty((x.shape[0], cout), dtype=out_dtype, device=self.dev)
+        self.ctx.conv(None, 1, self.s.PREC_BF16, x, w, b, y, cout, residual=residual)
+        return y
+
+    def forward(self, tables, h, taps=None):
+        """h: f32 [nc, c] -> f32 [nc, c]."""
+        t, ctx = self.torch, self.ctx
+        coords, plan = tables
+        x = t.empty(h.shape, dtype=t.bfloat16, device=self.dev)
+        ctx.layer_norm(h, 1e-6, x)
+        q = self._linear(x, self.q, t.bfloat16)
+        kv = self._linear(x, self.kv, t.bfloat16)
+        k, v = kv[:, :self.c], kv[:, self.c:]
+        ctx.qk_norm_rope(q, self.heads, self.q_gamma, q, k, self.heads, self.k_gamma, k, positions=coords[:, 1:],
+                         axis_pairs=self.pairs, theta=self.theta)
+        sel = None
+        if self.top:
+            sel = t.empty((plan.q_blocks, self.heads, self.top), dtype=t.int32, device=self.dev)
+            ctx.block_select(plan, q, k, self.heads, self.heads, sel, keep_local=True)
+        a = t.empty_like(q)
+        ctx.block_attention(plan, q, k, v, self.heads, self.heads, a, sel=sel)
+        if taps is not None:
+            taps.update(x=x, q=q, k=k, v=v, sel=sel, a=a)
+        return self._linear(a, self.out, t.float32, residual=h)
+
+
+def attention_params(c: int, heads: int, seed: int = 0) -> dict:
+    """Seeded random parameters of a CoarseAttention layer, Linears (Cout, Cin)."""
+    s = 90000 + 100 * seed
+
+    def lin(cout, k):
+        return dict(w=workloads.normal((cout, c), s + k, float(np.sqrt(1.0 / c))),
+                    b=workloads.normal((cout,), s + k + 1, 0.05))
+
+    d = c // heads
+    return dict(q=lin(c, 1), kv=lin(2 * c, 3), out=lin(c, 5), q_gamma=workloads.normal((heads, d), s + 7, 0.1) + 1.0,
+                k_gamma=workloads.normal((heads, d), s + 8, 0.1) + 1.0)

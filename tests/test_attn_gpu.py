@@ -20,7 +20,9 @@ import pytest
 import torch
 
 import s3dsp
+import slat
 import workloads
+from gates import gate
 
 pytestmark = pytest.mark.gpu
 
@@ -546,6 +548,14 @@ def test_attention_reports_a_block_that_is_not_there(ctx):
         ctx.check()
 
 
+def test_attention_refuses_to_write_over_its_inputs(ctx):
+    q, k, v = (randn((128, 64), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan([0, 128])
+    for bad in (q, k, v):
+        with pytest.raises(s3dsp.S3dError, match="overlap"):
+            ctx.block_attention(plan, q, k, v, 1, 1, bad)
+
+
 def test_attention_is_deterministic_and_plans_are_reusable(ctx):
     lens = [1111, 30, 2049]
     n = sum(lens)
@@ -696,45 +706,47 @@ def test_sm_limit_changes_nothing(ctx):
 # ---------------------------------------------------------------------------------------------------
 # together: a self-attention layer on the coarse rows of the SLat generator
 # ---------------------------------------------------------------------------------------------------
-def test_together_as_the_middle_of_the_sparse_stages(ctx):
-    """The four operators between the projections (s3dsp_conv), as SlatSparse.forward's `mid` runs them, every
-    step against its definition on the step's own inputs."""
-    coords = np.concatenate([workloads.ellipsoid_shell(24, 0), workloads.ellipsoid_shell(20, 1, batch=1)])
-    dcoords = torch.from_numpy(np.ascontiguousarray(coords)).cuda()
-    heads, d, top = 12, 64, 3
-    w = heads * d
-    h = ctx.hash_build(dcoords)
-    tables = ctx.slat_tables(h)
-    nc = tables.nc
-    coarse = torch.empty((nc, 4), dtype=torch.int32, device="cuda")
-    ctx.slat_tables_export(tables, coarse_coords=coarse)
-    lens = torch.bincount(coarse[:, 0].long(), minlength=2).tolist()
-    assert sum(lens) == nc and min(lens) > 300
-    x = randn((nc, w), 1, torch.bfloat16)
-    wp, ref = [], []
-    for s, (cin, cout) in enumerate(((w, 3 * w), (w, w))):
-        wt = randn((cout, cin), 100 + s, scale=cin ** -0.5)
-        dst = torch.empty(ctx.packed_bytes(s3dsp.PREC_BF16, 1, cin, cout), dtype=torch.uint8, device="cuda")
-        ctx.weights_pack(wt, s3dsp.LAYOUT_LINEAR, 1, cin, cout, s3dsp.PREC_BF16, dst)
-        wp.append(dst)
-        ref.append(wt)
-    plan = ctx.attn_plan(offsets(lens))
-    qkv = torch.empty((nc, 3 * w), dtype=torch.bfloat16, device="cuda")
-    ctx.conv(None, 1, s3dsp.PREC_BF16, x, wp[0], None, qkv, 3 * w)
-    _, _, gq, gk, buf = _chain_data(lens, heads, d, top, 9, plan)
-    _chain(ctx, plan, qkv, coarse[:, 1:], gq, gk, buf, heads, d)
-    y = torch.empty((nc, w), dtype=torch.float32, device="cuda")
-    ctx.conv(None, 1, s3dsp.PREC_BF16, buf["out"], wp[1], None, y, w, residual=x)
+@pytest.mark.parametrize("top", [0, 3])
+def test_together_in_the_middle_of_the_sparse_stages(ctx, top):
+    """slat.CoarseAttention as SlatSparse.forward's mid at the generator's width, two objects: every step against its
+    definition on the step's own inputs, and the layer as a whole within the BF16 gate."""
+    coords = np.concatenate([workloads.ellipsoid_shell(32, 0), workloads.ellipsoid_shell(24, 1, batch=1)])
+    device = torch.device("cuda", 0)
+    heads, c = 16, slat.MODEL_CH
+    d = c // heads
+    params = slat.attention_params(c, heads)
+    layer = slat.CoarseAttention(s3dsp, ctx, params, heads, device, top=top)
+    net = slat.SlatSparse(s3dsp, ctx, slat.slat_params(), s3dsp.PREC_BF16, device)
+    tb = slat.SlatTablesDev(s3dsp, ctx, torch.from_numpy(np.ascontiguousarray(coords)).cuda(), torch)
+    tables = layer.tables(tb)
+    pos, plan = tables[0][:, 1:], tables[1]
+    lens = torch.bincount(tables[0][:, 0].long()).tolist()
+    assert sum(lens) == tb.nc == plan.n_q and min(lens) > 300
+    t, seen = {}, {}
+
+    def mid(h):
+        seen["h"] = h.clone()
+        seen["y"] = layer.forward(tables, h, taps=t)
+        return seen["y"]
+
+    out = net.forward(tb, randn((tb.nf, slat.IN_CH), 1), net.mods_to_device(slat.slat_mods()), mid=mid)
     ctx.check()
-    assert float((qkv.double() - x.double() @ ref[0].to(torch.bfloat16).double().T).norm() / qkv.double().norm()) < 1e-2
-    for name, g, src in (("q", gq, qkv[:, :w]), ("k", gk, qkv[:, w:2 * w])):
-        t = src.double().reshape(nc, heads, d)
-        t = (t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * g.double()).reshape(nc, w)
-        want, size = turned(t, coarse[:, 1:], heads, [d // 6] * 3, 1e4, False, False)
-        within(buf[name], want, size * 26 * F32, unit(torch.bfloat16))
-    assert torch.equal(buf["sel"].cpu(), chosen(buf["q"], buf["k"], lens, lens, heads, heads, top, True))
-    v = qkv[:, 2 * w:]
-    check(buf["out"], buf["q"], buf["k"], v, lens, lens, heads, heads, d ** -0.5, buf["sel"])
-    check(buf["dense"], buf["q"], buf["k"], v, lens, lens, heads, heads, d ** -0.5)
-    want = buf["out"].double() @ ref[1].to(torch.bfloat16).double().T + x.double()
-    assert float((y.double() - want).norm() / want.norm()) < 1e-2
+    assert out.shape == (tb.nf, slat.OUT_CH) and torch.isfinite(out).all()
+
+    w = {k: (torch.from_numpy(params[k]["w"]).cuda().to(torch.bfloat16).double(), torch.from_numpy(params[k]["b"]).cuda().double())
+         for k in ("q", "kv", "out")}
+    x = torch.nn.functional.layer_norm(seen["h"].double(), (c,), eps=1e-6)
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+    gate(rel(t["x"], x), 1e-2, "layer norm")
+    lin = {k: t["x"].double() @ w[k][0].T + w[k][1] for k in ("q", "kv")}
+    gate(rel(t["v"], lin["kv"][:, c:]), 1e-2, "v")
+    heads_of = {"q": lin["q"], "k": lin["kv"][:, :c]}
+    for name in ("q", "k"):
+        g = torch.from_numpy(params[name + "_gamma"]).cuda().double()
+        a = heads_of[name].reshape(-1, heads, d)
+        a = (a / (a.square().mean(-1, keepdim=True) + 1e-6).sqrt() * g).reshape(-1, c)
+        gate(rel(t[name], turned(a, pos, heads, [d // 6] * 3, 1e4, False, False)[0]), 1e-2, name)
+    if top:
+        assert torch.equal(t["sel"].cpu(), chosen(t["q"], t["k"], lens, lens, heads, heads, top, True))
+    check(t["a"], t["q"], t["k"], t["v"], lens, lens, heads, heads, d ** -0.5, t["sel"])
+    gate(rel(seen["y"], t["a"].double() @ w["out"][0].T + w["out"][1] + seen["h"].double()), 1e-2, "layer")
