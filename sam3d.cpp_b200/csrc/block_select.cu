@@ -12,13 +12,19 @@
 //
 //   block_mean_kernel   one pass over q and k (memory bound): a warp lane owns eight columns, eight
 //                       warps share the block's rows, f64 sums joined in warp order
-//   block_score_kernel  scores of 32 query blocks x 64 key blocks of one sequence and head, a tile
-//                       product in f64 (the f64 pipe bounds it: 64 FMAs a cycle and SM), written as
+//   block_score_kernel  scores of 32 query blocks x 128 key blocks of one sequence and head, a tile
+//                       product in f64 (bound by the f64 pipe, 64 FMAs a cycle and SM), written as
 //                       64-bit keys whose unsigned order is the scores'
 //   top_warp_kernel     one warp per (query block, head): the top-th largest key by bisection, the
 //                       keys' upper halves in registers; the chosen indices in ascending order
 //   top_block_kernel    the same with one CTA per row and the keys in shared memory, for sequences
 //                       of more key blocks than a warp's registers take
+//
+// 65,500 rows, 16 heads of 64, bf16, lists of 32 (one B200): 142 us, of which the means 54 (268 MB
+// at 5.0 TB/s), the scores 55, the lists 30. Scores in f32 with an error bound, and f64 only where
+// the bound leaves a list in doubt: scores 37, lists 40, 135 us in all; at 28,000 and 1,900 rows
+// 70 and 27 us where this takes 66 and 25. Means with the 16-bit values taken to f64 by integer
+// instructions, or with a row's columns read by neighbouring CTAs: 54 and 61 us.
 #include "s3dsp_internal.h"
 
 using namespace s3dsp;
@@ -154,8 +160,9 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
 
 // A warp owns 32 query blocks x 32 key blocks as 4 x 4 f64 MMAs: eight shared
 // loads feed sixteen of them. (Scalar FMAs run at the same rate but need a
-// shared load each: 90 us with 4 x 4 register blocks where this takes 46.) Every
-// score is the same sequence of MMA steps, so that equal blocks have equal scores.
+// shared load each: 90 us with 4 x 4 register blocks where this takes 55, for
+// 512 x 1,024 blocks and 16 heads of 64.) Every score is the same sequence of
+// MMA steps, so that equal blocks have equal scores.
 __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreParams p) {
     // two stages of kTileD columns of the query rows and, below them, the key rows
     extern __shared__ __align__(16) double stage[][kTileQ + kTileK][kScoreLd];

@@ -295,6 +295,50 @@ def test_block_select_equal_blocks(ctx, n, copies):
         assert (sel[..., 1:] > sel[..., :-1]).all()
 
 
+@pytest.mark.parametrize("n", [64 * 20, 64 * 50, 64 * 700, 64 * 1500])
+@pytest.mark.parametrize("q0,k0,q1,k1", [
+    (1.0, 2.0**20, 1.0, 2.0**-10),      # apart by less than f32 keeps
+    (1.0, -2.0**20, 2.0**-20, 2.0**10),
+    (2.0**100, 2.0**100, 2.0**100, 2.0**80),     # beyond f32's range
+    (2.0**100, -2.0**100, 2.0**100, 2.0**100),   # beyond it in the middle of a sum
+    (2.0**-140, 2.0**100, 2.0**-149, 2.0**60),   # subnormal means
+    (2.0**-70, 2.0**-70, 2.0**-70, 2.0**-79),    # subnormal products
+])
+def test_block_select_close_and_extreme_scores(ctx, n, q0, k0, q1, k1):
+    """Scores q0 k0 + q1 k1 r for a permutation r of the blocks: exact in f64, equal, infinite or 0 in f32."""
+    blocks = n // 64
+    q, k = torch.zeros((200, 64), device="cuda"), torch.zeros((n, 64), device="cuda")
+    r = torch.from_numpy(np.random.default_rng(n).permutation(blocks).astype(np.float32))
+    q[:, 3], q[:, 40], k[:, 3] = q0, q1, k0
+    k[:, 40] = (r * k1).repeat_interleave(64).cuda()
+    plan = ctx.attn_plan([0, 200], [0, n])
+    for top in (1, 9, 33):
+        sel = torch.empty((plan.q_blocks, 1, top), dtype=torch.int32, device="cuda")
+        ctx.block_select(plan, q, k, 1, 1, sel)
+        assert torch.equal(sel.cpu(), chosen(q, k, [200], [n], 1, 1, top, False))
+
+
+@pytest.mark.parametrize("n,inf", [(64 * 30, False), (64 * 30, True), (64 * 1100, True)])
+@pytest.mark.parametrize("top", [1, 2, 3, 20])
+def test_block_select_keep_local_short_lists(ctx, n, inf, top):
+    """The own blocks come first, the lower one in a list of one; with infinite means beside them too."""
+    q, k = randn((n, 64), 5, torch.bfloat16), randn((n, 64), 6, torch.bfloat16)
+    if inf:
+        k[64 * 7:64 * 7 + 10, 5] = float("inf")
+        k[64 * 9:64 * 9 + 10, 5] = -float("inf")
+        k[64 * 11:64 * 11 + 10, 5] = float("nan")
+    plan = ctx.attn_plan([0, n])
+    sel = torch.empty((plan.q_blocks, 1, top), dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, 1, 1, sel, keep_local=True)
+    score = q.double().reshape(-1, 128, 64).mean(1) @ k.double().reshape(-1, 64, 64).mean(1).T
+    score = torch.where(score.isnan(), -torch.inf, score).cpu().numpy()
+    for b in range(n // 128):
+        c = np.arange(n // 64)
+        own = c // 2 == b
+        order = np.lexsort((c, np.where(own, 0, -score[b]), ~own))  # own first, then by score, then by index
+        assert (np.sort(order[:top]) == sel[b, 0].cpu().numpy()).all()
+
+
 @pytest.mark.parametrize("top", [1, 31, 33, 64, 129, 500])
 @pytest.mark.parametrize("n", [64 * 640, 64 * 1100])
 def test_block_select_list_lengths(ctx, n, top):
