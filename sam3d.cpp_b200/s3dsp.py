@@ -687,6 +687,12 @@ class Context:
               ptr(windows), windows.shape[0], ptr(scatter), ptr(out))
 
     # ---- attention over voxel tokens ----------------------------------------
+    def _here(self, *tensors):
+        """All of them (None aside) on the context's device."""
+        for t in tensors:
+            if t is not None and t.get_device() != self.device:
+                raise S3dError(S3D_INVALID_ARGUMENT, f"a tensor on {t.device} in a call on device {self.device}")
+
     @staticmethod
     def _positions(positions, axis_pairs, n):
         """(address, row stride, axes, host axis_pairs) of int32 positions [n, >= axes]."""
@@ -709,6 +715,7 @@ class Context:
         xp, xs = _rows(x, "x")
         yp, ys = _rows(out, "out")
         pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
+        self._here(x, positions, out)
         _call(load().s3dsp_rope, self.handle, xp, dtype_code(x), n, xs, heads, d, pos, pst, axes, pairs, theta,
               (ROPE_HALF if half else 0) | (ROPE_INVERSE if inverse else 0), yp, dtype_code(out), ys)
 
@@ -723,6 +730,8 @@ class Context:
         kp = kop = None
         ks = kos = 0
         flags = ROPE_HALF if half else 0
+        if (k is None) != (k_out is None):
+            raise S3dError(S3D_INVALID_ARGUMENT, "k and k_out: both or neither")
         if k is not None:
             _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
             _same("rows of q and k", n, k.shape[0])
@@ -734,9 +743,10 @@ class Context:
         if (q_gamma is not None and q_gamma.dim() == 1) or (k_gamma is not None and k_gamma.dim() == 1):
             flags |= QK_GAMMA_SHARED
         pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
-        _call(load().s3dsp_qk_norm_rope, self.handle, qp, qs, heads, self._gamma(q_gamma, heads, d, flags), kp, ks,
-              kv_heads, self._gamma(k_gamma, kv_heads, d, flags), dtype_code(q), n, d, eps, pos, pst, axes, pairs, theta,
-              flags, qop, qos, kop, kos, dtype_code(q_out))
+        qg, kg = self._gamma(q_gamma, heads, d, flags), self._gamma(k_gamma, kv_heads, d, flags)
+        self._here(q, q_gamma, q_out, k, k_gamma, k_out, positions)
+        _call(load().s3dsp_qk_norm_rope, self.handle, qp, qs, heads, qg, kp, ks, kv_heads, kg, dtype_code(q), n, d, eps,
+              pos, pst, axes, pairs, theta, flags, qop, qos, kop, kos, dtype_code(q_out))
 
     @staticmethod
     def _gamma(g, heads: int, d: int, flags: int):
@@ -787,6 +797,7 @@ class Context:
         top = self._lists(sel, plan, heads)
         qp, qs = _rows(q, "q")
         kp, ks = _rows(k, "k")
+        self._here(q, k, sel)
         _call(load().s3dsp_block_select, self.handle, plan.handle, qp, qs, heads, kp, ks, kv_heads, dtype_code(q), d,
               top, int(keep_local), sel.data_ptr())
 
@@ -800,6 +811,7 @@ class Context:
             raise S3dError(S3D_INVALID_ARGUMENT, f"types of q, v and out differ: {q.dtype}, {v.dtype}, {out.dtype}")
         top = 0 if sel is None else self._lists(sel, plan, heads)
         (qp, qs), (kp, ks), (vp, vs), (op, os_) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
+        self._here(q, k, v, out, sel)
         _call(load().s3dsp_block_attention, self.handle, plan.handle, qp, qs, heads, kp, ks, vp, vs, kv_heads,
               dtype_code(q), d, d ** -0.5 if scale is None else scale, ptr(sel), top, op, os_)
 

@@ -170,3 +170,23 @@ def test_binding_refuses():
             f()
             pytest.fail(f"call {i} was accepted")
 
+
+
+def test_binding_refuses_tensors_elsewhere():
+    c, x = Ctx(), torch.zeros(64, 512, dtype=torch.bfloat16)
+    c.device = 0
+    sel = torch.zeros(1, 8, 4, dtype=torch.int32)
+    for f in (
+        lambda: c.rope(x, POS, 8, x, [10, 10, 10]),
+        lambda: c.qk_norm_rope(x, 8, torch.ones(64), x),
+        lambda: c.block_select(Plan, x, x, 8, 8, sel),
+        lambda: c.block_attention(Plan, x, x, x, 8, 8, x.clone(), sel=sel),
+    ):
+        with pytest.raises(s3dsp.S3dError, match="a tensor on cpu"):
+            f()
+
+
+def test_binding_refuses_k_without_its_output():
+    c, x = Ctx(), torch.zeros(64, 512, dtype=torch.bfloat16)
+    with pytest.raises(s3dsp.S3dError, match="k_out"):
+        c.qk_norm_rope(x, 8, None, x, x, 8)
