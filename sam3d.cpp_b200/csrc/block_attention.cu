@@ -52,6 +52,7 @@ constexpr float kSlack = kF16 ? 8.f : 24.f;
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
+constexpr int kJoinRows = 8192;
 
 struct AttnParams {
     const int4* q_blocks;
@@ -65,7 +66,7 @@ struct AttnParams {
     int64_t q_stride;
     void* out;
     int64_t out_stride;
-    int tile_rows;   // most rows of a tile
+    int tiles, tile_rows;  // most rows of a tile
     float* part_o;   // [tiles][chunks][tile_rows][D] unnormalised sums
     float2* part_ml; // [tiles][chunks][tile_rows] their row maximum and sum
     uint32_t* status;
@@ -615,19 +616,22 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
     }
 }
 
-// Joins the chunks of a tile's rows: sums weighed by 2^(c (m_z - max m)). One
-// CTA per row: warp w adds chunks w, w + 8, ..., D / 32 columns per lane, and the
-// warps' sums are added in order. A chunk without blocks has m = -inf and is
-// not read.
-constexpr int kJoinWarps = 8;
-template <int D, bool kF16>
+// Joins the chunks of a tile's rows: sums weighed by 2^(c (m_z - max m)). kPer
+// warps per row: warp w of them adds chunks w, w + kPer, ..., D / 32 columns per
+// lane, and the warps' sums are added in order. A chunk without blocks has
+// m = -inf and is not read.
+constexpr int kJoinWarps = 8;  // of a CTA
+template <int D, bool kF16, int kPer>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const AttnParams p) {
-    __shared__ float sums[kJoinWarps][D + 1];
+    static_assert(kPer == 1 || kPer == kJoinWarps, "a row is a warp's or a CTA's");
+    __shared__ float sums[kPer == 1 ? 1 : kJoinWarps][D + 1];
     pdl_wait();
     pdl_trigger();
     constexpr int kC = D / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tile = blockIdx.x / p.tile_rows, row = blockIdx.x % p.tile_rows;
+    const int at_row = kPer == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
+    const int tile = at_row / p.tile_rows, row = at_row % p.tile_rows;
+    if (tile >= p.tiles) return;
     const int64_t step = p.tile_rows, at = (int64_t)tile * p.chunks * step + row;
     // every warp has all chunks' (m, l), chunk 32 i + lane in slot i
     float2 ml[kMaxChunks / 32];
@@ -652,11 +656,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const Attn
     if (!(top == -INFINITY)) {
 #pragma unroll
         for (int i = 0; i < kMaxChunks / 32; ++i) {
+            if (32 * i >= p.chunks) break;
             const float wl = ml[i].x == -INFINITY ? 0.f : exp2_hw((ml[i].x - top) * p.c);  // the chunk's weight
             const unsigned some = __ballot_sync(0xffffffffu, !(ml[i].x == -INFINITY));
-#pragma unroll
-            for (int b = 0; b < 32; b += kJoinWarps) {
-                const int src = b + warp;
+#pragma unroll 4
+            for (int src = kPer == 1 ? 0 : warp; src < min(32, p.chunks - 32 * i); src += kPer) {
                 const float w = __shfl_sync(0xffffffffu, wl, src), lz = __shfl_sync(0xffffffffu, ml[i].y, src);
                 if (!(some >> src & 1u)) continue;
                 l = fmaf(w, lz, l);
@@ -666,25 +670,33 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const Attn
             }
         }
     }
-#pragma unroll
-    for (int x = 0; x < kC; ++x) sums[warp][lane * kC + x] = acc[x];
-    if (lane == 0) sums[warp][D] = l;
-    __syncthreads();
-    if (threadIdx.x >= D / 2) return;
-    float a0 = 0.f, a1 = 0.f;
-    l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        a0 += sums[w][2 * threadIdx.x];
-        a1 += sums[w][2 * threadIdx.x + 1];
-        l += sums[w][D];
-    }
-    const bool none = l == 0.f;
-    const float inv = none ? 0.f : 1.f / l;
     const int64_t out_row = qb.x + row / p.pack;
     const int head = tile / p.n_qb * p.pack + row % p.pack;
-    reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D)[threadIdx.x] =
-        none ? 0u : pack2<kF16>(a0 * inv, a1 * inv);
+    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D);
+    if constexpr (kPer == 1) {
+        const bool none = l == 0.f;
+        const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+        for (int x = 0; x < kC; x += 2)
+            out[(lane * kC + x) / 2] = none ? 0u : pack2<kF16>(acc[x] * inv, acc[x + 1] * inv);
+    } else {
+#pragma unroll
+        for (int x = 0; x < kC; ++x) sums[warp][lane * kC + x] = acc[x];
+        if (lane == 0) sums[warp][D] = l;
+        __syncthreads();
+        if (threadIdx.x >= D / 2) return;
+        float a0 = 0.f, a1 = 0.f;
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            a0 += sums[w][2 * threadIdx.x];
+            a1 += sums[w][2 * threadIdx.x + 1];
+            l += sums[w][D];
+        }
+        const bool none = l == 0.f;
+        const float inv = none ? 0.f : 1.f / l;
+        out[threadIdx.x] = none ? 0u : pack2<kF16>(a0 * inv, a1 * inv);
+    }
 }
 
 // [rows][cols] 16-bit rows, tiles of box_rows x 64 columns with the 128-byte swizzle
@@ -732,7 +744,14 @@ cudaError_t launch(s3dsp_context* ctx, dim3 grid, const CUtensorMap& q, const CU
     e = launch_pdl(block_attention_kernel<D, kF16>, grid, dim3(Cfg<D>::kThreads), Cfg<D>::smem(p.sel ? p.top : 0),
                    ctx->stream, q, k, v, p);
     if (e != cudaSuccess || p.chunks == 1) return e;
-    return launch_pdl(join_chunks_kernel<D, kF16>, dim3(grid.x / p.chunks * p.tile_rows), dim3(32 * kJoinWarps), 0,
+    // A CTA per row where they all fit the SMs at once, else a warp per row: 64
+    // tiles of 128 rows, 18 chunks: 89 us for the call with a warp, 119 with a CTA;
+    // 84 tiles, 3 chunks: 26 and 67.
+    const int64_t rows = (int64_t)p.tiles * p.tile_rows;
+    const dim3 block(32 * kJoinWarps);
+    if (rows <= 8 * (int64_t)ctx->sm_count)
+        return launch_pdl(join_chunks_kernel<D, kF16, kJoinWarps>, dim3((unsigned)rows), block, 0, ctx->stream, p);
+    return launch_pdl(join_chunks_kernel<D, kF16, 1>, dim3((unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), block, 0,
                       ctx->stream, p);
 }
 
@@ -789,11 +808,13 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // several CTAs share a tile's list: chunks of equal length, by what the
     // lists hold together, so that they fill the slots about once however the
     // lengths differ. A chunk has at least kMinChunk blocks, and the split has
-    // to save kMinSaved: a block takes a CTA about 0.9 us, the joining kernel
-    // and its traffic about 8. (8 rows over 92k keys, 4 key heads: 527 us
-    // without, 58 with. Sharing only the tiles of a last, half empty wave was
-    // measured too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on
-    // an SM runs 1.2x as fast as one of two.)
+    // to save the time of kMinSaved blocks, and of one more per kJoinRows rows of
+    // partial sums: a block takes a CTA about 0.7 us (d = 64), the joining kernel
+    // about 6 and its traffic. (8 rows over 92k keys, 4 key heads: 527 us without,
+    // 56 with; 2,000 rows over 20,000, 4 heads: 203 and 89; 1,024 over 2,048, 8
+    // heads: 29 and 25; 1,024 over 1,024: 18 and 22, not split. Sharing only the
+    // tiles of a last, half empty wave was measured too, 720 tiles of 119 blocks:
+    // 304 us against 290. A CTA alone on an SM runs 1.2x as fast as one of two.)
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > 0x3fffffff) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "too many query blocks times heads");
     const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
@@ -804,7 +825,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
         chunk = ((d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) + lists - 1) / (lists > 0 ? lists : 1);
         if (chunk < kMinChunk) chunk = kMinChunk;
         if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
-        if (longest - chunk >= kMinSaved) chunks = (longest + chunk - 1) / chunk;
+        const int64_t parts = (longest + chunk - 1) / chunk;
+        if (longest - chunk >= kMinSaved + tiles * plan->max_q_rows * pack * parts / kJoinRows) chunks = parts;
     }
     CUtensorMap qm, km, vm;
     S3DSP_TRY(encode_q(&qm, q, plan->n_q, heads, d, q_stride, pack, f16, error, error_capacity));
@@ -823,6 +845,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.chunk = (int)chunk;
     p.chunks = (int)chunks;
     p.tile_rows = plan->max_q_rows * pack;
+    p.tiles = (int)tiles;
     p.c = scale * 1.4426950408889634f;
     p.q = q;
     p.q_stride = q_stride;

@@ -475,6 +475,25 @@ def test_block_attention(ctx, lens, klens, heads, kv, d, top, pad, dt):
     assert (out[:, heads * d:] == 7.0).all()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,klens,heads,kv,d,top", [
+    ([700, 0, 600, 3], [5000, 70, 40, 0], 4, 2, 64, 0),
+    ([700, 0, 600, 3], [5000, 70, 40, 0], 4, 2, 64, 60),
+    ([1280], [6000], 4, 4, 128, 0),
+    ([101] * 13, [2000 + 64 * i for i in range(13)], 3, 1, 128, 0),  # rows to join that are no multiple of eight
+])
+def test_attention_split_lists_of_many_rows(ctx, lens, klens, heads, kv, d, top, dt):
+    """Few tiles of many rows and long lists: several CTAs a list, the rows joined by a warp each."""
+    q = randn((sum(lens), heads * d), 1, DT[dt])
+    k, v = randn((sum(klens), kv * d), 2, DT[dt]), randn((sum(klens), kv * d), 3, DT[dt])
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    sel = lists(plan, heads, top, lens, klens, 4) if top else None
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, kv, out, sel=sel)
+    ctx.check()
+    check(out, q, k, v, lens, klens, heads, kv, d ** -0.5, sel)
+
+
 @pytest.mark.parametrize("top", [0, 12])
 @pytest.mark.parametrize("scale,size", [(1.0, 3.0), (0.001, 1.0), (4.0, 3.0), (1e-4, 0.1)])
 def test_attention_peaked_and_flat(ctx, scale, size, top):
