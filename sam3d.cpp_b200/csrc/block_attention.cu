@@ -2,9 +2,9 @@
 // rows of its listed key blocks (64 rows each), or over its whole sequence.
 //
 // One CTA per (query block of 128 rows, head); short blocks of grouped heads
-// share a tile, and where there are few tiles their lists are split over CTAs
-// and joined by a second kernel. The row maximum and sum run along with the
-// blocks (online softmax), so scores never leave the SM:
+// share a tile; where there are few tiles, or a few long ones, lists are split
+// over CTAs and joined by a second kernel. The row maximum and sum run along with
+// the blocks (online softmax), so scores never leave the SM:
 //
 //   key warp        K tiles by TMA into a ring; S = Q K^T (tcgen05, f32 in TMEM)
 //   value warp      V tiles by TMA into a ring; O += P V with P read from TMEM
@@ -34,6 +34,7 @@
 //            the FMA pipe (a polynomial): 851 us with one in eight, 894 with two. Two threads per row, or
 //            two groups of softmax warps per CTA: 909, 896. One warp for all MMAs: 868.
 //   d = 128  74 heads, 523 us, 1,215 TFLOP/s (0.72): MMAs and barriers alone 456 us
+#include <algorithm>
 #include <cmath>
 
 #include "tc_common.cuh"
@@ -53,20 +54,25 @@ constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at lea
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
 constexpr int kJoinRows = 8192;
+constexpr int64_t kMaxPartBytes = 1 << 28;  // partial sums of long lists among many
 
 struct AttnParams {
     const int4* q_blocks;
     const int32_t* sel;  // [n_qb][heads][top], or nullptr
     int top, heads, per_kv;
     int pack;   // heads of a group that share a tile: tile row r is query row r / pack, head r % pack
-    int n_qb;   // tile t: query block t % n_qb, heads from (t / n_qb) * pack
-    int chunk, chunks;  // CTAs that share a tile's list, and list entries of each
+    int n_qb;
+    // Tiles whose lists are split come first: tile t of them has query block t % n_long (counted in
+    // `order`), heads from (t / n_long) * pack, and `chunks` CTAs with `chunk` list entries each. Tile t of
+    // the rest: query block n_long + t % (n_qb - n_long), heads from t / (n_qb - n_long) * pack.
+    const int* order;  // nullptr: as they are
+    int n_long, chunk, chunks, split_ctas;
     float c;    // scale * log2(e)
     const void* q;
     int64_t q_stride;
     void* out;
     int64_t out_stride;
-    int tiles, tile_rows;  // most rows of a tile
+    int tiles, tile_rows;  // split tiles; most rows of a tile
     float* part_o;   // [tiles][chunks][tile_rows][D] unnormalised sums
     float2* part_ml; // [tiles][chunks][tile_rows] their row maximum and sum
     uint32_t* status;
@@ -276,10 +282,11 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
         if (warp == kValueWarp) prefetch_map(&vmap);
     }
     pdl_wait();
-    const bool split = p.chunks > 1;
-    const int tile = split ? (int)blockIdx.x / p.chunks : (int)blockIdx.x;
+    const bool split = (int)blockIdx.x < p.split_ctas;
+    const int tile = split ? (int)blockIdx.x / p.chunks : (int)blockIdx.x - p.split_ctas;
     const int first = split ? (int)blockIdx.x % p.chunks * p.chunk : 0;
-    const int bq = tile % p.n_qb, h = tile / p.n_qb * p.pack;
+    const int of = split ? p.n_long : p.n_qb - p.n_long, at_qb = tile % of + (split ? 0 : p.n_long);
+    const int bq = p.order ? __ldg(p.order + at_qb) : at_qb, h = tile / of * p.pack;
     // the list's first entries and the block's table entry are read together
     const int32_t* sel = p.sel ? p.sel + ((int64_t)bq * p.heads + h) * p.top : nullptr;
     int e = -1;
@@ -641,7 +648,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const Attn
         const int z = 32 * i + lane;
         ml[i] = z < p.chunks ? p.part_ml[z * step + at] : make_float2(-INFINITY, 0.f);
     }
-    const int4 qb = p.q_blocks[tile % p.n_qb];
+    const int at_qb = tile % p.n_long;
+    const int4 qb = p.q_blocks[p.order ? p.order[at_qb] : at_qb];
     if (row >= (qb.y & kAttnRowsMask) * p.pack) return;
 #pragma unroll
     for (int i = 0; i < kMaxChunks / 32; ++i) top = max3(top, ml[i].x, ml[i].x);
@@ -671,7 +679,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks_kernel(const Attn
         }
     }
     const int64_t out_row = qb.x + row / p.pack;
-    const int head = tile / p.n_qb * p.pack + row % p.pack;
+    const int head = tile / p.n_long * p.pack + row % p.pack;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D);
     if constexpr (kPer == 1) {
         const bool none = l == 0.f;
@@ -804,30 +812,49 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     int pack = 1;
     if (!d_sel)
         while (group % (2 * pack) == 0 && 2 * pack * plan->max_q_rows <= kQ) pack *= 2;
-    // Where the tiles leave half or more of the CTA slots (two per SM) empty,
-    // several CTAs share a tile's list: chunks of equal length, by what the
-    // lists hold together, so that they fill the slots about once however the
-    // lengths differ. A chunk has at least kMinChunk blocks, and the split has
-    // to save the time of kMinSaved blocks, and of one more per kJoinRows rows of
-    // partial sums: a block takes a CTA about 0.7 us (d = 64), the joining kernel
-    // about 6 and its traffic. (8 rows over 92k keys, 4 key heads: 527 us without,
-    // 56 with; 2,000 rows over 20,000, 4 heads: 203 and 89; 1,024 over 2,048, 8
-    // heads: 29 and 25; 1,024 over 1,024: 18 and 22, not split. Sharing only the
-    // tiles of a last, half empty wave was measured too, 720 tiles of 119 blocks:
-    // 304 us against 290. A CTA alone on an SM runs 1.2x as fast as one of two.)
+    // Several CTAs share a tile's list in chunks of equal length where the tiles
+    // leave half or more of the CTA slots (two per SM) empty, or where a few lists
+    // are far longer than the rest: chunks by what the lists hold together, so that
+    // they fill the slots about once. Lists of a chunk or less stay whole (with a
+    // selection all are taken for long). A chunk has at least kMinChunk blocks, and
+    // the split has to save the time of kMinSaved blocks, and of one more per
+    // kJoinRows rows of partial sums: a block takes a CTA about 0.7 us (d = 64), the
+    // joining kernel about 6 and its traffic. Without and with the split: 8 rows
+    // over 92k keys, 4 key heads, 527 and 53 us; 2,000 rows over 20,000, 4 heads, 203
+    // and 89; 1,024 over 2,048, 8 heads, 29 and 25; 1,024 over 1,024, 18 and 22 (not
+    // split); eight sequences of 1,000 rows, one over 20,000 keys, the others over
+    // 100, 257 and 97. Sharing only the tiles of a last, half empty wave was measured
+    // too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on an SM runs
+    // 1.2x as fast as one of two.
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > 0x3fffffff) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "too many query blocks times heads");
     const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
-    int64_t chunk = longest, chunks = 1;
+    const int64_t per_block = heads / pack;  // tiles of a query block
+    const int64_t work = (d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * per_block;  // blocks in all lists
+    int64_t chunk, last = longest;
     if (tiles <= slots / 2) {
         // sum over the lists of ceil(length / chunk) <= (their sum) / chunk + their number
-        const int64_t lists = slots / (heads / pack) - plan->n_qb;
-        chunk = ((d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) + lists - 1) / (lists > 0 ? lists : 1);
-        if (chunk < kMinChunk) chunk = kMinChunk;
-        if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
-        const int64_t parts = (longest + chunk - 1) / chunk;
-        if (longest - chunk >= kMinSaved + tiles * plan->max_q_rows * pack * parts / kJoinRows) chunks = parts;
+        const int64_t lists = slots / per_block - plan->n_qb;
+        chunk = (work / per_block + lists - 1) / (lists > 0 ? lists : 1);
+    } else {
+        // a few long lists among many: they end within a slot's share of the work, and one chunk more
+        chunk = (work + slots - 1) / slots;
+        last -= chunk;
     }
+    if (chunk < kMinChunk) chunk = kMinChunk;
+    if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
+    const int64_t shares = longest > chunk ? (longest + chunk - 1) / chunk : 1;
+    int64_t n_long = plan->n_qb;  // query blocks whose lists are longer than a chunk
+    if (!d_sel) {
+        const int4* seq = std::partition_point(plan->by_length, plan->by_length + plan->n_seq,
+                                               [&](const int4& s) { return s.x > chunk; });
+        n_long = seq == plan->by_length ? 0 : seq[-1].y;
+    }
+    const int64_t split_tiles = n_long * per_block, row_bytes = d * sizeof(float) + sizeof(float2);
+    const int64_t all = split_tiles * shares, filled = all < work / chunk + split_tiles ? all : work / chunk + split_tiles;
+    const int64_t tile_rows = plan->max_q_rows * pack;
+    const bool split = last - chunk >= kMinSaved + filled * tile_rows / kJoinRows &&
+                       (tiles <= slots / 2 || all * tile_rows * row_bytes <= kMaxPartBytes);
     CUtensorMap qm, km, vm;
     S3DSP_TRY(encode_q(&qm, q, plan->n_q, heads, d, q_stride, pack, f16, error, error_capacity));
     // a plan without key rows lists nothing: its maps are never read through
@@ -842,10 +869,16 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.per_kv = group;
     p.pack = pack;
     p.n_qb = plan->n_qb;
-    p.chunk = (int)chunk;
-    p.chunks = (int)chunks;
-    p.tile_rows = plan->max_q_rows * pack;
-    p.tiles = (int)tiles;
+    p.tile_rows = (int)tile_rows;
+    p.chunks = 1;
+    if (split) {
+        p.order = d_sel ? nullptr : plan->order;
+        p.n_long = (int)n_long;
+        p.chunk = (int)chunk;
+        p.chunks = (int)shares;
+        p.tiles = (int)split_tiles;
+        p.split_ctas = (int)all;
+    }
     p.c = scale * 1.4426950408889634f;
     p.q = q;
     p.q_stride = q_stride;
@@ -853,13 +886,13 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.out_stride = out_stride;
     p.status = ctx->d_status;
     char* parts = nullptr;
-    if (chunks > 1) {
-        const size_t rows = (size_t)tiles * chunks * p.tile_rows;
-        S3DSP_CUDA(malloc_async(&parts, rows * (d * sizeof(float) + sizeof(float2)), ctx->stream), "chunk sums");
+    if (split) {
+        const size_t rows = (size_t)all * tile_rows;
+        S3DSP_CUDA(malloc_async(&parts, rows * row_bytes, ctx->stream), "chunk sums");
         p.part_o = reinterpret_cast<float*>(parts);
         p.part_ml = reinterpret_cast<float2*>(parts + rows * d * sizeof(float));
     }
-    const dim3 grid((unsigned)(tiles * chunks));
+    const dim3 grid((unsigned)(split ? all + tiles - split_tiles : tiles));
     cudaError_t e = d == 64 ? (f16 ? launch<64, true>(ctx, grid, qm, km, vm, p) : launch<64, false>(ctx, grid, qm, km, vm, p))
                             : (f16 ? launch<128, true>(ctx, grid, qm, km, vm, p)
                                    : launch<128, false>(ctx, grid, qm, km, vm, p));

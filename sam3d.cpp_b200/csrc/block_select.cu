@@ -25,6 +25,8 @@
 // the bound leaves a list in doubt: scores 37, lists 40, 135 us in all; at 28,000 and 1,900 rows
 // 70 and 27 us where this takes 66 and 25. Means with the 16-bit values taken to f64 by integer
 // instructions, or with a row's columns read by neighbouring CTAs: 54 and 61 us.
+#include <algorithm>
+
 #include "s3dsp_internal.h"
 
 using namespace s3dsp;
@@ -495,10 +497,12 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
         if (m > max_kb) max_kb = m;
     }
     auto* plan = new (std::nothrow) s3dsp_attn_plan();
-    // one upload: q_blocks int4, k_blocks int2, groups int2, first_kb int
-    const size_t bytes = (size_t)nqb * (sizeof(int4) + sizeof(int2) + sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
+    // one upload: q_blocks int4, k_blocks int2, groups int2, first_kb int, order int
+    const size_t bytes = (size_t)nqb * (sizeof(int4) + sizeof(int2) + 2 * sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
     char* host = plan ? static_cast<char*>(::operator new(bytes, std::nothrow)) : nullptr;
-    if (!host) {
+    if (host) plan->by_length = static_cast<int4*>(::operator new(((size_t)n_seq + 1) * sizeof(int4), std::nothrow));
+    if (!host || !plan->by_length) {
+        ::operator delete(host);
         delete plan;
         return fail(error, error_capacity, S3D_OUT_OF_MEMORY, "plan allocation");
     }
@@ -506,10 +510,13 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     int2* kb = reinterpret_cast<int2*>(qb + nqb);
     int2* groups = kb + nkb;
     int* first_kb = reinterpret_cast<int*>(groups + nqb);
+    int* order = first_kb + nqb;
+    int4* seqs = plan->by_length;  // {key blocks, sequence, first query block, query blocks} until it is sorted
     int64_t iq = 0, ik = 0, ig = 0;
     for (int64_t s = 0; s < n_seq; ++s) {
         const int64_t q0 = h_q_offsets[s], ql = h_q_offsets[s + 1] - q0, k0 = ko[s], kl = ko[s + 1] - k0;
         const int64_t nb = ceil_div(ql, kAttnQRows);
+        seqs[s] = make_int4((int)ceil_div(kl, kAttnKRows), (int)s, (int)iq, (int)nb);
         for (int64_t b = 0; b < nb; ++b) {
             const int64_t left = ql - b * kAttnQRows;
             if (b % kAttnGroupRows == 0)
@@ -525,6 +532,13 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
             kb[ik++] = make_int2((int)(k0 + b * kAttnKRows), (int)(left < kAttnKRows ? left : kAttnKRows));
         }
     }
+    std::sort(seqs, seqs + n_seq, [](const int4& a, const int4& b) { return a.x != b.x ? a.x > b.x : a.y < b.y; });
+    int64_t io = 0;
+    for (int64_t s = 0; s < n_seq; ++s) {
+        for (int b = 0; b < seqs[s].w; ++b) order[io++] = seqs[s].z + b;
+        seqs[s].y = (int)io;
+    }
+    plan->n_seq = (int)n_seq;
     plan->device = ctx->device;
     plan->self = self;
     plan->n_q = nq, plan->n_k = nk;
@@ -538,6 +552,7 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     }
     ::operator delete(host);
     if (e != cudaSuccess) {
+        ::operator delete(plan->by_length);
         delete plan;
         return cuda_fail(error, error_capacity, e, "plan upload");
     }
@@ -545,6 +560,7 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     plan->k_blocks = reinterpret_cast<int2*>(plan->q_blocks + nqb);
     plan->groups = plan->k_blocks + nkb;
     plan->first_kb = reinterpret_cast<int*>(plan->groups + nqb);
+    plan->order = plan->first_kb + nqb;
     *out = plan;
     return S3D_OK;
 }
@@ -555,6 +571,7 @@ extern "C" S3DSP_API void s3dsp_attn_plan_free(s3dsp_context* ctx, s3dsp_attn_pl
         cudaSetDevice(ctx->device);
         cudaFreeAsync(plan->mem, ctx->stream);
     }
+    ::operator delete(plan->by_length);
     delete plan;
 }
 

@@ -93,6 +93,9 @@ struct s3dsp_attn_plan {
     int2* k_blocks = nullptr;        // [n_kb] {first row, rows}
     int2* groups = nullptr;          // [n_groups] {first query block, up to kAttnGroupRows blocks of one sequence}
     int* first_kb = nullptr;         // [n_qb] first key block of the block's sequence
+    int* order = nullptr;            // [n_qb] query blocks, those of the longest key sequences first
+    int4* by_length = nullptr;       // host [n_seq], longest first: {key blocks, query blocks so far, -, -}
+    int n_seq = 0;
 };
 
 namespace s3dsp {

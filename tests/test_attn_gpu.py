@@ -494,6 +494,23 @@ def test_attention_split_lists_of_many_rows(ctx, lens, klens, heads, kv, d, top,
     check(out, q, k, v, lens, klens, heads, kv, d ** -0.5, sel)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,klens,heads,kv,d", [
+    ([500] * 8, [100] * 3 + [9000] + [0, 64, 65, 1], 8, 8, 64),             # one long sequence among many tiles
+    ([1] * 90 + [100, 3, 0], [64] * 90 + [20000, 9000, 8000], 16, 4, 128),  # and tiles of few rows
+    ([700, 130, 400, 128, 900], [3000, 40, 12000, 9000, 500], 12, 6, 64),   # several, in no order
+])
+def test_attention_long_lists_among_many(ctx, lens, klens, heads, kv, d, dt):
+    """More tiles than CTA slots, a few of them far longer: those are split, the others are not."""
+    q = randn((sum(lens), heads * d), 1, DT[dt])
+    k, v = randn((sum(klens), kv * d), 2, DT[dt]), randn((sum(klens), kv * d), 3, DT[dt])
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, kv, out)
+    ctx.check()
+    check(out, q, k, v, lens, klens, heads, kv, d ** -0.5)
+
+
 @pytest.mark.parametrize("top", [0, 12])
 @pytest.mark.parametrize("scale,size", [(1.0, 3.0), (0.001, 1.0), (4.0, 3.0), (1e-4, 0.1)])
 def test_attention_peaked_and_flat(ctx, scale, size, top):
