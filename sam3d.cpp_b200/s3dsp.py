@@ -259,15 +259,15 @@ def _int32s(values: tuple):
 
 
 def _rows(t, name: str):
-    """(address, row stride) of a 2-D tensor whose columns are contiguous."""
+    """(address, row stride, rows, columns) of a 2-D tensor whose columns are contiguous."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: rows of contiguous columns are wanted")
-    return t.data_ptr(), (stride[0] if shape[0] > 1 else max(stride[0], shape[1]))
+    n, w = shape
+    return t.data_ptr(), (stride[0] if n > 1 else max(stride[0], w)), n, w
 
 
-def _head_dim(t, heads: int, name: str) -> int:
-    w = t.shape[-1]
+def _head_dim(w: int, heads: int, name: str) -> int:
     if heads <= 0 or w % heads:
         raise S3dError(S3D_INVALID_ARGUMENT, f"{name}: {w} columns are no {heads} heads")
     return w // heads
@@ -699,21 +699,20 @@ class Context:
         axes = len(axis_pairs)
         if axes == 0:
             return None, 0, 0, None
-        import torch
-        if positions is None or positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[0] != n \
-                or positions.shape[1] < axes:
-            raise S3dError(S3D_INVALID_ARGUMENT, f"positions: int32 [{n}, >= {axes}] rows are wanted")
-        return *_rows(positions, "positions"), axes, _int32s(tuple(axis_pairs))
+        if positions is not None:
+            p, stride, rows, cols = _rows(positions, "positions")
+            if rows == n and cols >= axes and str(positions.dtype) == "torch.int32":
+                return p, stride, axes, _int32s(tuple(axis_pairs))
+        raise S3dError(S3D_INVALID_ARGUMENT, f"positions: int32 [{n}, >= {axes}] rows are wanted")
 
     def rope(self, x, positions, heads: int, out, axis_pairs, theta: float = 10000.0, half: bool = False,
              inverse: bool = False):
         """out = x [n, heads * d] with every head turned by positions (int32
         [n, axes]); axis_pairs: pairs of each axis. Rows may be strided."""
-        d = _head_dim(x, heads, "x")
-        _same("x and out", x.shape, out.shape)
-        n = x.shape[0]
-        xp, xs = _rows(x, "x")
-        yp, ys = _rows(out, "out")
+        xp, xs, n, w = _rows(x, "x")
+        yp, ys, ny, wy = _rows(out, "out")
+        d = _head_dim(w, heads, "x")
+        _same("x and out", (n, w), (ny, wy))
         pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
         self._here(x, positions, out)
         _call(load().s3dsp_rope, self.handle, xp, dtype_code(x), n, xs, heads, d, pos, pst, axes, pairs, theta,
@@ -723,23 +722,23 @@ class Context:
                      eps: float = 1e-6, positions=None, axis_pairs=(), theta: float = 10000.0, half: bool = False):
         """RMS norm of every head of q (and k) with weights f32 [heads, d] (or
         [d] for all heads, or None), then the rotation (axis_pairs () : none)."""
-        n, d = q.shape[0], _head_dim(q, heads, "q")
-        _same("q and q_out", q.shape, q_out.shape)
-        qp, qs = _rows(q, "q")
-        qop, qos = _rows(q_out, "q_out")
+        qp, qs, n, w = _rows(q, "q")
+        qop, qos, no, wo = _rows(q_out, "q_out")
+        d = _head_dim(w, heads, "q")
+        _same("q and q_out", (n, w), (no, wo))
         kp = kop = None
         ks = kos = 0
         flags = ROPE_HALF if half else 0
         if (k is None) != (k_out is None):
             raise S3dError(S3D_INVALID_ARGUMENT, "k and k_out: both or neither")
         if k is not None:
-            _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
-            _same("rows of q and k", n, k.shape[0])
+            kp, ks, nk, wk = _rows(k, "k")
+            kop, kos, no, wo = _rows(k_out, "k_out")
+            _same("head dimensions", d, _head_dim(wk, kv_heads, "k"))
+            _same("rows of q and k", n, nk)
+            _same("k and k_out", (nk, wk), (no, wo))
             _same("types of q and k", q.dtype, k.dtype)
-            _same("k and k_out", k.shape, k_out.shape)
             _same("output types", q_out.dtype, k_out.dtype)
-            kp, ks = _rows(k, "k")
-            kop, kos = _rows(k_out, "k_out")
         if (q_gamma is not None and q_gamma.dim() == 1) or (k_gamma is not None and k_gamma.dim() == 1):
             flags |= QK_GAMMA_SHARED
         pos, pst, axes, pairs = self._positions(positions, axis_pairs, n)
@@ -754,8 +753,7 @@ class Context:
         if g is None:
             return None
         want = (d,) if flags & QK_GAMMA_SHARED else (heads, d)
-        import torch
-        if g.dtype != torch.float32 or tuple(g.shape) != want or not g.is_contiguous():
+        if g.shape != want or str(g.dtype) != "torch.float32" or not g.is_contiguous():
             raise S3dError(S3D_INVALID_ARGUMENT, f"gamma: contiguous float32 {want} is wanted")
         return g.data_ptr()
 
@@ -773,30 +771,28 @@ class Context:
         return AttnPlan(self, h.value)
 
     @staticmethod
-    def _attn_rows(plan: AttnPlan, q, heads: int, k, kv_heads: int):
-        d = _head_dim(q, heads, "q")
-        _same("head dimensions", d, _head_dim(k, kv_heads, "k"))
-        _same("types of q and k", q.dtype, k.dtype)
-        if q.shape[0] < plan.n_q or k.shape[0] < plan.n_k:
-            raise S3dError(S3D_INVALID_ARGUMENT, f"the plan spans {plan.n_q} query rows and {plan.n_k} key rows")
-        return d
-
-    @staticmethod
     def _lists(sel, plan: AttnPlan, heads: int) -> int:
         """The length of the lists in sel (int32 [plan.q_blocks, heads, top])."""
-        import torch
         shape = sel.shape
-        if len(shape) != 3 or shape[0] != plan.q_blocks or shape[1] != heads or sel.dtype != torch.int32 or \
+        if len(shape) != 3 or shape[0] != plan.q_blocks or shape[1] != heads or str(sel.dtype) != "torch.int32" or \
                 not sel.is_contiguous():
             raise S3dError(S3D_INVALID_ARGUMENT, f"sel: contiguous int32 [{plan.q_blocks}, {heads}, top] is wanted")
         return shape[2]
 
+    @staticmethod
+    def _spans(plan: AttnPlan, n_q: int, n_k: int):
+        if n_q < plan.n_q or n_k < plan.n_k:
+            raise S3dError(S3D_INVALID_ARGUMENT, f"the plan spans {plan.n_q} query rows and {plan.n_k} key rows")
+
     def block_select(self, plan: AttnPlan, q, k, heads: int, kv_heads: int, sel, keep_local: bool = False):
         """sel (device int32 [plan.q_blocks, heads, top]) = the key blocks with the largest scores."""
-        d = self._attn_rows(plan, q, heads, k, kv_heads)
+        qp, qs, nq, wq = _rows(q, "q")
+        kp, ks, nk, wk = _rows(k, "k")
+        d = _head_dim(wq, heads, "q")
+        _same("head dimensions", d, _head_dim(wk, kv_heads, "k"))
+        _same("types of q and k", q.dtype, k.dtype)
+        self._spans(plan, nq, nk)
         top = self._lists(sel, plan, heads)
-        qp, qs = _rows(q, "q")
-        kp, ks = _rows(k, "k")
         self._here(q, k, sel)
         _call(load().s3dsp_block_select, self.handle, plan.handle, qp, qs, heads, kp, ks, kv_heads, dtype_code(q), d,
               top, int(keep_local), sel.data_ptr())
@@ -804,13 +800,18 @@ class Context:
     def block_attention(self, plan: AttnPlan, q, k, v, heads: int, kv_heads: int, out, scale: float | None = None,
                         sel=None):
         """out = softmax(scale q k^T over the listed key blocks (sel None: all)) v; scale None: 1 / sqrt(d)."""
-        d = self._attn_rows(plan, q, heads, k, kv_heads)
-        _same("k and v", k.shape, v.shape)
-        _same("q and out", q.shape, out.shape)
-        if not q.dtype == v.dtype == out.dtype:
-            raise S3dError(S3D_INVALID_ARGUMENT, f"types of q, v and out differ: {q.dtype}, {v.dtype}, {out.dtype}")
+        qp, qs, nq, wq = _rows(q, "q")
+        kp, ks, nk, wk = _rows(k, "k")
+        vp, vs, nv, wv = _rows(v, "v")
+        op, os_, no, wo = _rows(out, "out")
+        d = _head_dim(wq, heads, "q")
+        _same("head dimensions", d, _head_dim(wk, kv_heads, "k"))
+        _same("k and v", (nk, wk), (nv, wv))
+        _same("q and out", (nq, wq), (no, wo))
+        if not q.dtype == k.dtype == v.dtype == out.dtype:
+            raise S3dError(S3D_INVALID_ARGUMENT, f"types differ: {q.dtype}, {k.dtype}, {v.dtype}, {out.dtype}")
+        self._spans(plan, nq, nk)
         top = 0 if sel is None else self._lists(sel, plan, heads)
-        (qp, qs), (kp, ks), (vp, vs), (op, os_) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(out, "out")
         self._here(q, k, v, out, sel)
         _call(load().s3dsp_block_attention, self.handle, plan.handle, qp, qs, heads, kp, ks, vp, vs, kv_heads,
               dtype_code(q), d, d ** -0.5 if scale is None else scale, ptr(sel), top, op, os_)
