@@ -61,11 +61,11 @@ struct AttnParams {
     const int32_t* sel;  // [n_qb][heads][top], or nullptr
     int top, heads, per_kv;
     int pack;   // heads of a group that share a tile: tile row r is query row r / pack, head r % pack
-    int n_qb;
-    // Tiles whose lists are split come first: tile t of them has query block t % n_long (counted in
-    // `order`), heads from (t / n_long) * pack, and `chunks` CTAs with `chunk` list entries each. Tile t of
-    // the rest: query block n_long + t % (n_qb - n_long), heads from t / (n_qb - n_long) * pack.
-    const int* order;  // nullptr: as they are
+    int n_qb, per_block;  // query blocks, tiles of each: heads / pack
+    // Tiles whose lists are split come first: the n_long first query blocks of `order`, head by head, and
+    // `chunks` CTAs each with `chunk` list entries. Then the other tiles: query block by query block of
+    // `order`, or without one head by head.
+    const int* order;
     int n_long, chunk, chunks, split_ctas;
     float c;    // scale * log2(e)
     const void* q;
@@ -285,8 +285,10 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
     const bool split = (int)blockIdx.x < p.split_ctas;
     const int tile = split ? (int)blockIdx.x / p.chunks : (int)blockIdx.x - p.split_ctas;
     const int first = split ? (int)blockIdx.x % p.chunks * p.chunk : 0;
-    const int of = split ? p.n_long : p.n_qb - p.n_long, at_qb = tile % of + (split ? 0 : p.n_long);
-    const int bq = p.order ? __ldg(p.order + at_qb) : at_qb, h = tile / of * p.pack;
+    const bool by_block = p.order && !split;
+    const int of = by_block ? p.per_block : split ? p.n_long : p.n_qb;
+    const int at_qb = by_block ? p.n_long + tile / of : tile % of;
+    const int bq = p.order ? __ldg(p.order + at_qb) : at_qb, h = (by_block ? tile % of : tile / of) * p.pack;
     // the list's first entries and the block's table entry are read together
     const int32_t* sel = p.sel ? p.sel + ((int64_t)bq * p.heads + h) * p.top : nullptr;
     int e = -1;
@@ -870,9 +872,14 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.pack = pack;
     p.n_qb = plan->n_qb;
     p.tile_rows = (int)tile_rows;
+    // Where the lists' lengths differ, the longest start first, with all their heads, so that short ones
+    // fill the end: objects of 15,159, 4,211, 8,190 and 2,777 rows, 16 heads, 1,665 us against 1,800 in the
+    // sequences' order, head by head, and 1,775 with the longest of each head first. Equal lengths stay in
+    // their order, which reads a head's rows close together (forty objects of 300: 63 against 65).
+    if (!d_sel && (split || 4 * (int64_t)longest * plan->n_qb > 5 * plan->sum_kb)) p.order = plan->order;
+    p.per_block = (int)per_block;
     p.chunks = 1;
     if (split) {
-        p.order = d_sel ? nullptr : plan->order;
         p.n_long = (int)n_long;
         p.chunk = (int)chunk;
         p.chunks = (int)shares;

@@ -499,6 +499,7 @@ def test_attention_split_lists_of_many_rows(ctx, lens, klens, heads, kv, d, top,
     ([500] * 8, [100] * 3 + [9000] + [0, 64, 65, 1], 8, 8, 64),             # one long sequence among many tiles
     ([1] * 90 + [100, 3, 0], [64] * 90 + [20000, 9000, 8000], 16, 4, 128),  # and tiles of few rows
     ([700, 130, 400, 128, 900], [3000, 40, 12000, 9000, 500], 12, 6, 64),   # several, in no order
+    ([128, 0, 1000, 64, 300, 1, 500], [100, 0, 1000, 64, 0, 1, 400], 12, 4, 128),  # none split, the longest first
 ])
 def test_attention_long_lists_among_many(ctx, lens, klens, heads, kv, d, dt):
     """More tiles than CTA slots, a few of them far longer: those are split, the others are not."""
