@@ -215,26 +215,15 @@ def prepare(case, seed):
     return s
 
 
-_contexts = {}
-
-
-def _context():
-    """The program's one context on this stream, made once."""
+def _handles(s):
+    """What a user's program of the framework keeps between calls: its context, the plan of the batch
+    and the output buffers."""
     here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sam3d.cpp_b200")
     if here not in sys.path:
         sys.path.insert(0, here)
     import s3dsp
-    stream = torch.cuda.current_stream().cuda_stream
-    if stream not in _contexts:
-        _contexts[stream] = s3dsp.Context(0)
-    return _contexts[stream]
-
-
-def _handles(s):
-    """What a user's program of the framework keeps between calls: its context, the plan of the batch
-    and the output buffers."""
     c = s["case"]
-    ctx = s["ctx"] = _context()
+    ctx = s["ctx"] = s3dsp.Context(0)
     new = lambda x, dt: torch.empty((x.shape[0], x.shape[1]), dtype=dt, device="cuda")  # noqa: E731
     if c["op"] in ("rope", "qk"):
         s["q_out"] = new(s["q"], DT[c["out"]])
