@@ -448,7 +448,7 @@ S3DSP_API s3d_status s3dsp_attn_plan_info(const s3dsp_attn_plan *plan, int64_t *
  * Means and scores are f64, so a list does not depend on the order of sums.
  * keep_local != 0 (self attention plans only): the key blocks of the query
  * block's own rows come first. d a multiple of 8 up to 256, any strides; a
- * sequence has at most 28,000 key blocks. */
+ * sequence with query rows has at most 28,000 key blocks. */
 S3DSP_API s3d_status s3dsp_block_select(s3dsp_context *ctx, const s3dsp_attn_plan *plan, const void *q,
                                         int64_t q_stride, int32_t heads, const void *k, int64_t k_stride,
                                         int32_t kv_heads, uint32_t dtype, int32_t d, int32_t top,

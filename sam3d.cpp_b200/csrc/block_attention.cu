@@ -830,7 +830,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // 1.2x as fast as one of two.
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
     if (tiles > 0x3fffffff) return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "too many query blocks times heads");
-    const int longest = d_sel ? (top < plan->max_kb ? top : plan->max_kb) : plan->max_kb;
+    const int longest = d_sel && top < plan->max_list ? top : plan->max_list;  // list of a query block, at most
     const int64_t per_block = heads / pack;  // tiles of a query block
     const int64_t work = (d_sel ? (int64_t)plan->n_qb * longest : plan->sum_kb) * per_block;  // blocks in all lists
     int64_t chunk, last = longest;
@@ -848,7 +848,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     const int64_t shares = longest > chunk ? (longest + chunk - 1) / chunk : 1;
     int64_t n_long = plan->n_qb;  // query blocks whose lists are longer than a chunk
     if (!d_sel) {
-        const int4* seq = std::partition_point(plan->by_length, plan->by_length + plan->n_seq,
+        const int4* seq = std::partition_point(plan->by_length, plan->by_length + plan->n_by_length,
                                                [&](const int4& s) { return s.x > chunk; });
         n_long = seq == plan->by_length ? 0 : seq[-1].y;
     }

@@ -512,11 +512,15 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     int* first_kb = reinterpret_cast<int*>(groups + nqb);
     int* order = first_kb + nqb;
     int4* seqs = plan->by_length;  // {key blocks, sequence, first query block, query blocks} until it is sorted
-    int64_t iq = 0, ik = 0, ig = 0;
+    int64_t iq = 0, ik = 0, ig = 0, is = 0;
     for (int64_t s = 0; s < n_seq; ++s) {
         const int64_t q0 = h_q_offsets[s], ql = h_q_offsets[s + 1] - q0, k0 = ko[s], kl = ko[s + 1] - k0;
         const int64_t nb = ceil_div(ql, kAttnQRows);
-        seqs[s] = make_int4((int)ceil_div(kl, kAttnKRows), (int)s, (int)iq, (int)nb);
+        if (nb > 0) {
+            const int blocks = (int)ceil_div(kl, kAttnKRows);
+            seqs[is++] = make_int4(blocks, (int)s, (int)iq, (int)nb);
+            if (blocks > plan->max_list) plan->max_list = blocks;
+        }
         for (int64_t b = 0; b < nb; ++b) {
             const int64_t left = ql - b * kAttnQRows;
             if (b % kAttnGroupRows == 0)
@@ -532,13 +536,13 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
             kb[ik++] = make_int2((int)(k0 + b * kAttnKRows), (int)(left < kAttnKRows ? left : kAttnKRows));
         }
     }
-    std::sort(seqs, seqs + n_seq, [](const int4& a, const int4& b) { return a.x != b.x ? a.x > b.x : a.y < b.y; });
+    std::sort(seqs, seqs + is, [](const int4& a, const int4& b) { return a.x != b.x ? a.x > b.x : a.y < b.y; });
     int64_t io = 0;
-    for (int64_t s = 0; s < n_seq; ++s) {
+    for (int64_t s = 0; s < is; ++s) {
         for (int b = 0; b < seqs[s].w; ++b) order[io++] = seqs[s].z + b;
         seqs[s].y = (int)io;
     }
-    plan->n_seq = (int)n_seq;
+    plan->n_by_length = (int)is;
     plan->device = ctx->device;
     plan->self = self;
     plan->n_q = nq, plan->n_k = nk;
@@ -615,9 +619,10 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
     const size_t es = dtype_size(dtype);
     if (((uintptr_t)q | (uintptr_t)k) & (es - 1))
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "pointer not aligned to its type");
-    if (plan->max_kb > kMaxKeys)
-        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "a sequence has %d key blocks (at most %d)",
-                    plan->max_kb, kMaxKeys);
+    const int longest = plan->max_list;  // key blocks of a row's sequence, at most
+    if (longest > kMaxKeys)
+        return fail(error, error_capacity, S3D_INVALID_ARGUMENT, "a sequence has %d key blocks (at most %d)", longest,
+                    kMaxKeys);
     S3DSP_CUDA(cudaSetDevice(ctx->device), "cudaSetDevice");
     static std::atomic<uint64_t> optin{0}, score_optin{0};
     S3DSP_CUDA(smem_optin((const void*)block_score_kernel, ctx->device, score_optin), "block_score_kernel");
@@ -625,8 +630,8 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
     double* means = nullptr;
     const size_t n_qm = (size_t)plan->n_qb * qw, n_km = (size_t)plan->n_kb * kw;
     // scores of as many heads at a time as kScoreBytes take (one at least)
-    const size_t row_bytes = (size_t)plan->n_qb * plan->max_kb * sizeof(unsigned long long);
-    const bool scored = plan->max_kb > top;
+    const size_t row_bytes = (size_t)plan->n_qb * longest * sizeof(unsigned long long);
+    const bool scored = longest > top;
     int64_t pass = scored && row_bytes * heads > kScoreBytes ? kScoreBytes / row_bytes : heads;
     if (pass < 1) pass = 1;
     const size_t score_bytes = scored ? row_bytes * pass : 0;
@@ -646,22 +651,22 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
     else
         vec ? mean(block_mean_kernel<__half, true>) : mean(block_mean_kernel<__half, false>);
     ScoreParams s = {plan->groups, plan->q_blocks, plan->first_kb, means, means + n_qm, (int)qw, (int)kw, plan->n_qb, d,
-                     heads, heads / kv_heads, top, keep_local, 0, 0, plan->max_kb,
+                     heads, heads / kv_heads, top, keep_local, 0, 0, longest,
                      reinterpret_cast<unsigned long long*>(means + n_qm + n_km), d_sel};
     for (int h0 = 0; h0 < heads && e == cudaSuccess; h0 += (int)pass) {
         s.head0 = h0;
         s.head_count = (int)(heads - h0 < pass ? heads - h0 : pass);
         if (scored)
             e = launch_pdl(block_score_kernel,
-                           dim3((unsigned)plan->n_groups, (unsigned)ceil_div(plan->max_kb, kTileK), (unsigned)s.head_count),
+                           dim3((unsigned)plan->n_groups, (unsigned)ceil_div(longest, kTileK), (unsigned)s.head_count),
                            dim3(kScoreThreads), kScoreSmem, ctx->stream, s);
         if (e != cudaSuccess) break;
         const int64_t items = (int64_t)plan->n_qb * s.head_count;
-        if (plan->max_kb <= 32 * kWarpKeys)
+        if (longest <= 32 * kWarpKeys)
             e = launch_pdl(top_warp_kernel, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, ctx->stream, s);
         else
             e = launch_pdl(top_block_kernel, dim3((unsigned)items), dim3(kTopThreads),
-                           (plan->max_kb + 1) * sizeof(unsigned long long), ctx->stream, s);
+                           (longest + 1) * sizeof(unsigned long long), ctx->stream, s);
     }
     const cudaError_t f = cudaFreeAsync(means, ctx->stream);
     if (e == cudaSuccess) e = f;

@@ -88,14 +88,15 @@ struct s3dsp_attn_plan {
     int max_q_rows = 0;              // most rows of a query block
     int n_qb = 0, n_kb = 0, n_groups = 0;
     int max_kb = 0;                  // most key blocks of a sequence
+    int max_list = 0;                // most key blocks of a sequence that has query rows
     void* mem = nullptr;
     int4* q_blocks = nullptr;        // [n_qb] {first row, rows | index in the sequence << 8, first key row, key rows}
     int2* k_blocks = nullptr;        // [n_kb] {first row, rows}
     int2* groups = nullptr;          // [n_groups] {first query block, up to kAttnGroupRows blocks of one sequence}
     int* first_kb = nullptr;         // [n_qb] first key block of the block's sequence
     int* order = nullptr;            // [n_qb] query blocks, those of the longest key sequences first
-    int4* by_length = nullptr;       // host [n_seq], longest first: {key blocks, query blocks so far, -, -}
-    int n_seq = 0;
+    int4* by_length = nullptr;       // host [n_by_length], longest first: {key blocks, query blocks so far, -, -}
+    int n_by_length = 0;             // sequences that have query rows
 };
 
 namespace s3dsp {

@@ -831,3 +831,39 @@ def test_together_in_the_middle_of_the_sparse_stages(ctx, top):
         assert torch.equal(t["sel"].cpu(), chosen(t["q"], t["k"], lens, lens, heads, heads, top, True))
     check(t["a"], t["q"], t["k"], t["v"], lens, lens, heads, heads, d ** -0.5, t["sel"])
     gate(rel(seen["y"], t["a"].double() @ w["out"][0].T + w["out"][1] + seen["h"].double()), 1e-2, "layer")
+
+
+# ---------------------------------------------------------------------------------------------------
+# batches whose longest key sequence has no query rows
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,klens,heads,kv,d", [
+    ([0, 1], [42000, 100], 16, 4, 128),                       # few tiles
+    ([0, 300], [6000, 200], 12, 12, 64),
+    ([0, 4000, 100], [6000, 300, 100], 16, 16, 64),           # more tiles than CTA slots
+    ([2, 0, 1], [9000, 90000, 64], 16, 4, 128),               # another list is split
+    ([500] * 7 + [0], [100] * 3 + [9000] + [0, 64, 65, 60000], 8, 8, 64),
+])
+def test_attention_longest_keys_without_queries(ctx, lens, klens, heads, kv, d, dt):
+    q = randn((sum(lens), heads * d), 1, DT[dt])
+    k, v = randn((sum(klens), kv * d), 2, DT[dt]), randn((sum(klens), kv * d), 3, DT[dt])
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    assert plan.max_k_blocks == max(-(-m // 64) for m in klens)
+    for top in (0, 5):
+        sel = lists(plan, heads, top, lens, klens, 4) if top else None
+        out = torch.full_like(q, 7.0)
+        ctx.block_attention(plan, q, k, v, heads, kv, out, sel=sel)
+        ctx.check()
+        check(out, q, k, v, lens, klens, heads, kv, d ** -0.5, sel)
+
+
+@pytest.mark.parametrize("lens,klens,top", [
+    ([0, 300], [64 * 1100, 3000], 5), ([200, 0, 5], [700, 64 * 28001, 64 * 20], 3), ([0, 300], [9000, 200], 5),
+])
+def test_block_select_longest_keys_without_queries(ctx, lens, klens, top):
+    """Key blocks that no query row sees count neither for the limit nor for the lists."""
+    q, k = randn((sum(lens), 128), 1, torch.bfloat16), randn((sum(klens), 128), 2, torch.bfloat16)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    sel = torch.full((plan.q_blocks, 2, top), -7, dtype=torch.int32, device="cuda")
+    ctx.block_select(plan, q, k, 2, 2, sel)
+    assert torch.equal(sel.cpu(), chosen(q, k, lens, klens, 2, 2, top, False))
