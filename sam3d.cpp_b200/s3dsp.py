@@ -625,6 +625,14 @@ class Context:
     def check(self):
         _call(load().s3dsp_context_check, self.handle)
 
+    def torch_stream(self):
+        """The context's stream as a torch stream."""
+        import torch
+        stream = load().s3dsp_context_stream(self.handle)
+        if not stream:
+            return torch.cuda.default_stream(self.device)
+        return torch.cuda.ExternalStream(stream, device=self.device)
+
     def fork(self):
         """CONTEXT_COPY_STREAMS: order the copy streams after the context's stream."""
         _call(load().s3dsp_context_fork, self.handle)

@@ -200,12 +200,18 @@ class CoarseAttention:
     pairs for each of x, y, z), attention over every coarse row of the row's
     object, or with `top` > 0 over the `top` blocks of 64 rows that
     s3dsp_block_select picks for each 128 query rows and head (the block of the
-    rows themselves among them). The objects of a batch are its sequences."""
+    rows themselves among them). The objects of a batch are its sequences.
+
+    Torch's part (allocations, the count of each object's rows) runs on the
+    context's stream too, whichever is current: torch reads what the library
+    has written, and buffers freed on return are reused in that order. Results
+    are that stream's; a caller on another one waits for it."""
 
     def __init__(self, s3dsp, ctx, params: dict, heads: int, device, top: int = 0, theta: float = 10000.0):
         import torch
         self.s, self.ctx, self.torch, self.dev = s3dsp, ctx, torch, device
         self.c, self.heads, self.top, self.theta = params["out"]["w"].shape[0], heads, top, theta
+        self.stream = ctx.torch_stream()
         self.pairs = [self.c // heads // 6] * 3
 
         def dev(a):
@@ -219,15 +225,17 @@ class CoarseAttention:
                              cin, cout, s3dsp.PREC_BF16, dst)
             return dst, dev(d["b"]), cout
 
-        self.q, self.kv, self.out = (lin(params[k]) for k in ("q", "kv", "out"))
-        self.q_gamma, self.k_gamma = dev(params["q_gamma"]), dev(params["k_gamma"])
+        with torch.cuda.stream(self.stream):
+            self.q, self.kv, self.out = (lin(params[k]) for k in ("q", "kv", "out"))
+            self.q_gamma, self.k_gamma = dev(params["q_gamma"]), dev(params["k_gamma"])
 
     def tables(self, tb: SlatTablesDev):
         """What a batch of objects needs, made once: the coarse coordinates and the attention plan."""
         t = self.torch
-        coords = t.empty((tb.nc, 4), dtype=t.int32, device=self.dev)
-        self.ctx.slat_tables_export(tb.tables, coarse_coords=coords)
-        rows = t.bincount(coords[:, 0].long()).cpu().numpy()  # coarse rows are sorted by object
+        with t.cuda.stream(self.stream):
+            coords = t.empty((tb.nc, 4), dtype=t.int32, device=self.dev)
+            self.ctx.slat_tables_export(tb.tables, coarse_coords=coords)
+            rows = t.bincount(coords[:, 0].long()).cpu().numpy()  # coarse rows are sorted by object
         return coords, self.ctx.attn_plan(np.concatenate([[0], np.cumsum(rows)]))
 
     def _linear(self, x, wbc, out_dtype, residual=None):
@@ -238,6 +246,10 @@ class CoarseAttention:
 
     def forward(self, tables, h, taps=None):
         """h: f32 [nc, c] -> f32 [nc, c]."""
+        with self.torch.cuda.stream(self.stream):
+            return self._forward(tables, h, taps)
+
+    def _forward(self, tables, h, taps):
         t, ctx = self.torch, self.ctx
         coords, plan = tables
         x = t.empty(h.shape, dtype=t.bfloat16, device=self.dev)

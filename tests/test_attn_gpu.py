@@ -867,3 +867,43 @@ def test_block_select_longest_keys_without_queries(ctx, lens, klens, top):
     sel = torch.full((plan.q_blocks, 2, top), -7, dtype=torch.int32, device="cuda")
     ctx.block_select(plan, q, k, 2, 2, sel)
     assert torch.equal(sel.cpu(), chosen(q, k, lens, klens, 2, 2, top, False))
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_coarse_attention_on_a_stream_that_is_not_current(ctx, own):
+    """tables() and forward() on a context whose stream is busy and not torch's current one (its own, or another torch
+    stream): the row counts are read after the coordinates are written, and buffers that torch hands out again
+    meanwhile are not the layer's."""
+    device = torch.device("cuda", 0)
+    coords = np.concatenate([workloads.ellipsoid_shell(24, b, batch=b) for b in range(3)])
+    d_coords = torch.from_numpy(np.ascontiguousarray(coords)).cuda()
+    heads, c = 4, 256
+    params = slat.attention_params(c, heads)
+    layer = slat.CoarseAttention(s3dsp, ctx, params, heads, device, top=3)
+    tb = slat.SlatTablesDev(s3dsp, ctx, d_coords, torch)
+    want_tables = layer.tables(tb)
+    h = randn((tb.nc, c), 1)
+    want = layer.forward(want_tables, h)
+    torch.cuda.synchronize()
+
+    stream = torch.cuda.Stream()
+    other = s3dsp.Context(0, stream=0 if own else stream.cuda_stream, flags=s3dsp.CONTEXT_OWN_STREAM if own else 0)
+    layer = slat.CoarseAttention(s3dsp, other, params, heads, device, top=3)
+    tb2 = slat.SlatTablesDev(s3dsp, other, d_coords, torch)
+    other.check()
+    junk = [torch.full((tb.nc, w), -1, dtype=torch.int32, device="cuda") for w in (4, c, c // 2)]
+    torch.cuda.synchronize()
+    del junk  # torch's stream gets these rows of -1 next
+    with torch.cuda.stream(layer.stream):
+        torch.cuda._sleep(20_000_000)
+    tables = layer.tables(tb2)
+    assert torch.equal(tables[0], want_tables[0])
+    assert (tables[1].n_q, tables[1].q_blocks) == (want_tables[1].n_q, want_tables[1].q_blocks)
+    for _ in range(3):
+        with torch.cuda.stream(layer.stream):
+            torch.cuda._sleep(20_000_000)
+        got = layer.forward(tables, h)
+        for w in (4, c // 2, c, 2 * c):  # torch's stream writes wherever it may
+            torch.full((tb.nc, w), 7, dtype=torch.int32, device="cuda")
+        other.check()
+        assert torch.equal(got, want)
