@@ -46,10 +46,14 @@ namespace {
 
 constexpr int kQ = kAttnQRows, kK = kAttnKRows;
 constexpr int kQPanel = kQ * 128, kKPanel = kK * 128;  // bytes of 64 columns of a Q / K / V tile
-// how far (in powers of two) a row's maximum may grow past the one in use: a
-// weight up to 2^24 is as exact in bf16 and f32 as one up to 1; f16 ends at 65,504
+// How far (in powers of two) a row's maximum may grow past the one in use.
+constexpr float kSlack = 8.f;
+// All weights carry a factor 2^kShift, which the division by their sum takes out
+// again. bf16: a weight is 1 at most, so that their sum with v ends where f32 does
+// for weights exp(s - max) (|v| times the rows 2^128), however the maximum grew.
+// f16: the largest is 2^8.
 template <bool kF16>
-constexpr float kSlack = kF16 ? 8.f : 24.f;
+constexpr float kShift = kF16 ? 0.f : -kSlack;
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
             F2 sum[2];
             for (int attempt = 0;; ++attempt) {
                 // (an infinite maximum makes its row NaN, as inf - inf does)
-                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m));
+                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m + kShift<kF16>));
                 float mx[2] = {m, m};
                 sum[0] = sum[1] = both(0.f);
 #pragma unroll
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
                 }
                 const float mt = max3(mx[0], mx[1], mx[1]);
                 // a NaN maximum counts as grown, and stays
-                const bool grown = !((mt - m) * p.c <= kSlack<kF16>) && !(mt == -INFINITY);
+                const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
                 if (attempt > 0 || !__any_sync(0xffffffffu, grown)) break;
                 const float to = grown ? mt : m;
                 const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;

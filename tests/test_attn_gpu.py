@@ -907,3 +907,29 @@ def test_coarse_attention_on_a_stream_that_is_not_current(ctx, own):
             torch.full((tb.nc, w), 7, dtype=torch.int32, device="cuda")
         other.check()
         assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------------------------------
+# the range of values and weights
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("grow", [7.5, 8.5, 16.0, 20.0, 23.9, 40.0])
+@pytest.mark.parametrize("lens,klens,heads,kv,d", [
+    ([130], [300], 2, 2, 64), ([130], [300], 2, 1, 128), ([1, 3], [6000, 200], 2, 2, 64),  # the last: a split list
+])
+def test_attention_of_large_values(ctx, lens, klens, heads, kv, d, grow):
+    """bf16 values whose plain sum with weights of at most 1 fits f32 (|v| times the keys up to 2^127), and a maximum
+    that grows by so many powers of two after the first block of keys."""
+    big = 2.0 ** 124 / max(klens)  # a normal value of more than 8 sigma does not come up
+    q = torch.zeros((sum(lens), heads * d), dtype=torch.bfloat16, device="cuda")
+    q[:, ::d] = 1.0
+    k = randn((sum(klens), kv * d), 2, torch.bfloat16, 0.25)
+    v = randn((sum(klens), kv * d), 3, torch.bfloat16, big)
+    at = 0
+    for m in klens:
+        k[at + 64:at + m, ::d] += grow * np.log(2.0)
+        at += m
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, kv, out, scale=1.0)
+    ctx.check()
+    check(out, q, k, v, lens, klens, heads, kv, 1.0)
