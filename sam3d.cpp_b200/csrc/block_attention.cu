@@ -51,9 +51,12 @@ constexpr float kSlack = 8.f;
 // All weights carry a factor 2^kShift, which the division by their sum takes out
 // again. bf16: a weight is 1 at most, so that their sum with v ends where f32 does
 // for weights exp(s - max) (|v| times the rows 2^128), however the maximum grew.
-// f16: the largest is 2^8.
+// f16, whose range is short: the largest weight is 2^15 (of 65,504), so that one
+// is exact to its 11 bits down to 2^-21 of the row's largest and lost only
+// below 2^-32 of it. Without the shift many keys of weight 2^-14 to 2^-25 beside a
+// single large one came out wrong by up to their whole sum.
 template <bool kF16>
-constexpr float kShift = kF16 ? 0.f : -kSlack;
+constexpr float kShift = kF16 ? 7.f : -kSlack;
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list

@@ -933,3 +933,31 @@ def test_attention_of_large_values(ctx, lens, klens, heads, kv, d, grow):
     ctx.block_attention(plan, q, k, v, heads, kv, out, scale=1.0)
     ctx.check()
     check(out, q, k, v, lens, klens, heads, kv, 1.0)
+
+
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("gap", [12.3, 17.7, 20.4, 23.6, 25.2, 29.5])
+@pytest.mark.parametrize("lens,klens,heads,kv,d", [
+    ([130], [4000], 2, 2, 64), ([130], [4000], 2, 1, 128), ([1, 3], [20000, 4000], 2, 2, 64),  # split lists
+    ([2000], [4000], 16, 4, 64), ([2000], [4000], 16, 4, 128),                                 # whole ones
+])
+def test_attention_f16_of_small_weights(ctx, lens, klens, heads, kv, d, gap, last):
+    """f16: one key (the first or the last) with a score far above the others', which are equal, and with value 0: the
+    others' weights, 2^-gap of its, all round the same way. A weight is off by u of it or 2^-25 2^-7 of the largest."""
+    q = torch.zeros((sum(lens), heads * d), dtype=torch.float16, device="cuda")
+    q[:, ::d] = 1.0
+    k = torch.zeros((sum(klens), kv * d), dtype=torch.float16, device="cuda")
+    v = randn((sum(klens), kv * d), 3, torch.float16, 0.25) + 1.0
+    at = 0
+    for m in klens:
+        one = at + (m - 1 if last else 0)
+        k[one, ::d], v[one] = gap * np.log(2.0), 0.0
+        at += m
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, kv, out, scale=1.0)
+    ctx.check()
+    want, (mass, size) = attention(q, k, v, lens, klens, heads, kv, 1.0)
+    u = unit(torch.float16)
+    tol = (mass * (u + 2 * (size * d * 2.0 ** -23 + 4 * 2.0 ** -22) + 16 * F32)).flatten(1)
+    within(out, want, tol + 2.0 ** -32 * float(v.abs().max()) * max(klens), u)
