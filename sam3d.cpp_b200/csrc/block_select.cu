@@ -41,7 +41,7 @@ constexpr int kScoreLd = kTileD + 4;                                // shared ro
 constexpr int kWarpKeys = 32;                                     // key blocks per lane of top_warp_kernel
 constexpr size_t kScoreSmem = 2 * sizeof(double) * (kTileQ + kTileK) * kScoreLd;  // four CTAs per SM
 constexpr int kMaxKeys = 28000;                                   // key blocks of a sequence: top_block_kernel's memory
-constexpr size_t kScoreBytes = (size_t)1 << 29;                   // scratch of scores that a pass over heads may take
+constexpr size_t kScoreBytes = (size_t)1 << 29;                   // scratch of scores that a pass may take
 
 template <typename T>
 __device__ __forceinline__ double to_d(T v);
@@ -134,15 +134,16 @@ __global__ void __launch_bounds__(kMeanThreads) block_mean_kernel(MeanParams p) 
 }
 
 struct ScoreParams {
-    const int2* groups;     // {first query block, blocks}: one sequence's
+    const int2* groups;     // {first query block, blocks}: one sequence's; those of this pass
     const int4* q_blocks;   // {first row, rows | index in the sequence << 8, first key row, key rows}
     const int* first_kb;    // [n_qb] first key block of the block's sequence
     const double* q_mean;
     const double* k_mean;
-    int qw, kw, n_qb, d, heads, per_kv, top, keep_local;
-    int head0, head_count;  // heads of this pass
-    int max_kb;             // keys of a row
-    unsigned long long* keys;  // [n_qb][head_count][max_kb]
+    int qw, kw, d, heads, per_kv, top, keep_local;
+    int block0, block_count;  // query blocks of this pass
+    int head0, head_count;    // heads of this pass
+    int max_kb;               // keys of a row
+    unsigned long long* keys;  // [block_count][head_count][max_kb]
     int32_t* sel;              // [n_qb][heads][top]
 };
 
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(kScoreThreads) block_score_kernel(const ScoreP
         if (r >= count) continue;
         // the key blocks of the query block's own rows come first
         const int own = p.keep_local ? ((qb0.y >> kAttnRowsBits) + r) * (kAttnQRows / kAttnKRows) : -2;
-        unsigned long long* row = p.keys + ((int64_t)(b0 + r) * p.head_count + blockIdx.z) * p.max_kb;
+        unsigned long long* row = p.keys + ((int64_t)(b0 + r - p.block0) * p.head_count + blockIdx.z) * p.max_kb;
 #pragma unroll
         for (int y = 0; y < 4; ++y)
 #pragma unroll
@@ -256,8 +257,8 @@ __global__ void __launch_bounds__(128) top_warp_kernel(const ScoreParams p) {
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (int64_t)p.n_qb * p.head_count) return;
-    const int b = (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
+    if (item >= (int64_t)p.block_count * p.head_count) return;
+    const int b = p.block0 + (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
     const int nkb = (p.q_blocks[b].w + kAttnKRows - 1) / kAttnKRows;
     int32_t* out = p.sel + ((int64_t)b * p.heads + h) * p.top;
     if (nkb <= p.top) {  // all of them
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kTopThreads) top_block_kernel(const ScoreParam
     pdl_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t item = blockIdx.x;
-    const int b = (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
+    const int b = p.block0 + (int)(item / p.head_count), h = p.head0 + (int)(item % p.head_count);
     const int nkb = (p.q_blocks[b].w + kAttnKRows - 1) / kAttnKRows;
     int32_t* out = p.sel + ((int64_t)b * p.heads + h) * p.top;
     if (nkb <= p.top) {
@@ -500,9 +501,13 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     // one upload: q_blocks int4, k_blocks int2, groups int2, first_kb int, order int
     const size_t bytes = (size_t)nqb * (sizeof(int4) + sizeof(int2) + 2 * sizeof(int)) + (size_t)nkb * sizeof(int2) + 16;
     char* host = plan ? static_cast<char*>(::operator new(bytes, std::nothrow)) : nullptr;
-    if (host) plan->by_length = static_cast<int4*>(::operator new(((size_t)n_seq + 1) * sizeof(int4), std::nothrow));
-    if (!host || !plan->by_length) {
+    if (host) {
+        plan->by_length = static_cast<int4*>(::operator new(((size_t)n_seq + 1) * sizeof(int4), std::nothrow));
+        plan->group_first = static_cast<int*>(::operator new(((size_t)nqb + 1) * sizeof(int), std::nothrow));
+    }
+    if (!host || !plan->by_length || !plan->group_first) {
         ::operator delete(host);
+        if (plan) ::operator delete(plan->by_length), ::operator delete(plan->group_first);
         delete plan;
         return fail(error, error_capacity, S3D_OUT_OF_MEMORY, "plan allocation");
     }
@@ -523,8 +528,10 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
         }
         for (int64_t b = 0; b < nb; ++b) {
             const int64_t left = ql - b * kAttnQRows;
-            if (b % kAttnGroupRows == 0)
+            if (b % kAttnGroupRows == 0) {
+                plan->group_first[ig] = (int)iq;
                 groups[ig++] = make_int2((int)iq, (int)(nb - b < kAttnGroupRows ? nb - b : kAttnGroupRows));
+            }
             plan->sum_kb += ceil_div(kl, kAttnKRows);
             if (plan->max_q_rows < left) plan->max_q_rows = (int)(left < kAttnQRows ? left : kAttnQRows);
             first_kb[iq] = (int)ik;
@@ -543,6 +550,7 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
         seqs[s].y = (int)io;
     }
     plan->n_by_length = (int)is;
+    plan->group_first[ig] = (int)nqb;
     plan->device = ctx->device;
     plan->self = self;
     plan->n_q = nq, plan->n_k = nk;
@@ -557,6 +565,7 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
     ::operator delete(host);
     if (e != cudaSuccess) {
         ::operator delete(plan->by_length);
+        ::operator delete(plan->group_first);
         delete plan;
         return cuda_fail(error, error_capacity, e, "plan upload");
     }
@@ -576,6 +585,7 @@ extern "C" S3DSP_API void s3dsp_attn_plan_free(s3dsp_context* ctx, s3dsp_attn_pl
         cudaFreeAsync(plan->mem, ctx->stream);
     }
     ::operator delete(plan->by_length);
+    ::operator delete(plan->group_first);
     delete plan;
 }
 
@@ -629,12 +639,15 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
     S3DSP_CUDA(smem_optin((const void*)top_block_kernel, ctx->device, optin), "top_block_kernel");
     double* means = nullptr;
     const size_t n_qm = (size_t)plan->n_qb * qw, n_km = (size_t)plan->n_kb * kw;
-    // scores of as many heads at a time as kScoreBytes take (one at least)
+    // scores of as many heads at a time as kScoreBytes take, or of one head and as many groups of query
+    // blocks (one at least: 32 rows of up to 28,000 keys are 7 MB)
     const size_t row_bytes = (size_t)plan->n_qb * longest * sizeof(unsigned long long);
     const bool scored = longest > top;
     int64_t pass = scored && row_bytes * heads > kScoreBytes ? kScoreBytes / row_bytes : heads;
     if (pass < 1) pass = 1;
-    const size_t score_bytes = scored ? row_bytes * pass : 0;
+    int64_t pass_blocks = plan->n_qb;
+    if (scored && row_bytes > kScoreBytes) pass_blocks = kScoreBytes / (longest * sizeof(unsigned long long));
+    const size_t score_bytes = scored ? row_bytes / plan->n_qb * pass_blocks * pass : 0;
     S3DSP_CUDA(malloc_async(&means, (n_qm + n_km) * sizeof(double) + score_bytes + 16, ctx->stream), "block scores");
     MeanParams m = {q, k, q_stride, k_stride, (int)qw, (int)kw, plan->n_qb, plan->n_kb, plan->q_blocks, plan->k_blocks,
                     means, means + n_qm};
@@ -650,23 +663,31 @@ extern "C" S3DSP_API s3d_status s3dsp_block_select(s3dsp_context* ctx, const s3d
         vec ? mean(block_mean_kernel<__nv_bfloat16, true>) : mean(block_mean_kernel<__nv_bfloat16, false>);
     else
         vec ? mean(block_mean_kernel<__half, true>) : mean(block_mean_kernel<__half, false>);
-    ScoreParams s = {plan->groups, plan->q_blocks, plan->first_kb, means, means + n_qm, (int)qw, (int)kw, plan->n_qb, d,
-                     heads, heads / kv_heads, top, keep_local, 0, 0, longest,
+    ScoreParams s = {plan->groups, plan->q_blocks, plan->first_kb, means, means + n_qm, (int)qw, (int)kw, d,
+                     heads, heads / kv_heads, top, keep_local, 0, 0, 0, 0, longest,
                      reinterpret_cast<unsigned long long*>(means + n_qm + n_km), d_sel};
-    for (int h0 = 0; h0 < heads && e == cudaSuccess; h0 += (int)pass) {
-        s.head0 = h0;
-        s.head_count = (int)(heads - h0 < pass ? heads - h0 : pass);
-        if (scored)
-            e = launch_pdl(block_score_kernel,
-                           dim3((unsigned)plan->n_groups, (unsigned)ceil_div(longest, kTileK), (unsigned)s.head_count),
-                           dim3(kScoreThreads), kScoreSmem, ctx->stream, s);
-        if (e != cudaSuccess) break;
-        const int64_t items = (int64_t)plan->n_qb * s.head_count;
-        if (longest <= 32 * kWarpKeys)
-            e = launch_pdl(top_warp_kernel, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, ctx->stream, s);
-        else
-            e = launch_pdl(top_block_kernel, dim3((unsigned)items), dim3(kTopThreads),
-                           (longest + 1) * sizeof(unsigned long long), ctx->stream, s);
+    const int* first = plan->group_first;
+    for (int g0 = 0, g1; g0 < plan->n_groups && e == cudaSuccess; g0 = g1) {
+        // whole groups, up to pass_blocks query blocks
+        g1 = (int)(std::upper_bound(first + g0 + 1, first + plan->n_groups + 1, first[g0] + pass_blocks) - first) - 1;
+        s.groups = plan->groups + g0;
+        s.block0 = first[g0];
+        s.block_count = first[g1] - first[g0];
+        for (int h0 = 0; h0 < heads && e == cudaSuccess; h0 += (int)pass) {
+            s.head0 = h0;
+            s.head_count = (int)(heads - h0 < pass ? heads - h0 : pass);
+            if (scored)
+                e = launch_pdl(block_score_kernel,
+                               dim3((unsigned)(g1 - g0), (unsigned)ceil_div(longest, kTileK), (unsigned)s.head_count),
+                               dim3(kScoreThreads), kScoreSmem, ctx->stream, s);
+            if (e != cudaSuccess) break;
+            const int64_t items = (int64_t)s.block_count * s.head_count;
+            if (longest <= 32 * kWarpKeys)
+                e = launch_pdl(top_warp_kernel, dim3((unsigned)ceil_div(items, 4)), dim3(128), 0, ctx->stream, s);
+            else
+                e = launch_pdl(top_block_kernel, dim3((unsigned)items), dim3(kTopThreads),
+                               (longest + 1) * sizeof(unsigned long long), ctx->stream, s);
+        }
     }
     const cudaError_t f = cudaFreeAsync(means, ctx->stream);
     if (e == cudaSuccess) e = f;

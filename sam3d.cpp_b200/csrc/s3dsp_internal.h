@@ -97,6 +97,7 @@ struct s3dsp_attn_plan {
     int* order = nullptr;            // [n_qb] query blocks, those of the longest key sequences first
     int4* by_length = nullptr;       // host [n_by_length], longest first: {key blocks, query blocks so far, -, -}
     int n_by_length = 0;             // sequences that have query rows
+    int* group_first = nullptr;      // host [n_groups + 1] first query block of each group, then n_qb
 };
 
 namespace s3dsp {

@@ -961,3 +961,36 @@ def test_attention_f16_of_small_weights(ctx, lens, klens, heads, kv, d, gap, las
     u = unit(torch.float16)
     tol = (mass * (u + 2 * (size * d * 2.0 ** -23 + 4 * 2.0 ** -22) + 16 * F32)).flatten(1)
     within(out, want, tol + 2.0 ** -32 * float(v.abs().max()) * max(klens), u)
+
+
+# ---------------------------------------------------------------------------------------------------
+# the scratch of a selection
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lens,klens,heads,top", [
+    ([330000], [64 * 28000], 2, 9),                             # cut inside a sequence, one head at a time
+    ([1] * 2500 + [300] + [1] * 2500, [64] * 2500 + [64 * 28000] + [200] * 2500, 1, 5),
+])
+def test_block_select_holds_at_most_512_mb_of_scores(ctx, lens, klens, heads, top):
+    """A head's scores (a row as long as the longest sequence for each query block) beyond that take several passes."""
+    d = 64
+    q, k = randn((sum(lens), heads * d), 1, torch.bfloat16), randn((sum(klens), heads * d), 2, torch.bfloat16)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    assert plan.q_blocks * plan.max_k_blocks * 8 > 1 << 29
+    sel = torch.full((plan.q_blocks, heads, top), -7, dtype=torch.int32, device="cuda")
+    ctx.check()
+    used = s3dsp.memory_stats(0, reset_high=True)["used"]
+    ctx.block_select(plan, q, k, heads, heads, sel)
+    ctx.check()
+    means = (plan.q_blocks + plan.k_blocks) * heads * d * 8
+    assert s3dsp.memory_stats(0)["used_high"] - used <= (1 << 29) + means + (1 << 16)
+    q0 = k0 = b0 = 0
+    for m, mk in zip(lens, klens):
+        nb, nk = -(-m // 128), -(-mk // 64)
+        if nk <= top:
+            want = torch.arange(top, device="cuda").where(torch.arange(top, device="cuda") < nk, -1).expand(nb, heads, top)
+        else:
+            mean = lambda x, rows: torch.stack([c.double().mean(0) for c in x.split(rows)]).reshape(-1, heads, d)  # noqa: E731
+            score = torch.einsum("bhd,chd->bhc", mean(q[q0:q0 + m], 128), mean(k[k0:k0 + mk], 64))
+            want = score.topk(top, dim=-1).indices.sort(dim=-1).values
+        assert torch.equal(sel[b0:b0 + nb].long(), want)
+        q0, k0, b0 = q0 + m, k0 + mk, b0 + nb
