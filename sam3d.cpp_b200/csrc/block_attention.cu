@@ -61,7 +61,7 @@ constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at lea
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
 constexpr int kJoinRows = 8192;
-constexpr int64_t kMaxPartBytes = 1 << 28;  // partial sums of long lists among many
+constexpr int64_t kMaxPartBytes = 1 << 28;  // partial sums of split lists
 
 struct AttnParams {
     const int4* q_blocks;
@@ -852,18 +852,26 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     }
     if (chunk < kMinChunk) chunk = kMinChunk;
     if (chunk < (longest + kMaxChunks - 1) / kMaxChunks) chunk = (longest + kMaxChunks - 1) / kMaxChunks;
-    const int64_t shares = longest > chunk ? (longest + chunk - 1) / chunk : 1;
-    int64_t n_long = plan->n_qb;  // query blocks whose lists are longer than a chunk
-    if (!d_sel) {
-        const int4* seq = std::partition_point(plan->by_length, plan->by_length + plan->n_by_length,
-                                               [&](const int4& s) { return s.x > chunk; });
-        n_long = seq == plan->by_length ? 0 : seq[-1].y;
+    // Every split tile has `shares` places, as many as the longest list takes. Where many lists are little
+    // longer than a chunk most of these stay empty: chunks are made longer until the places fit
+    // kMaxPartBytes (one list of 6,213 blocks beside 83 of 50, d = 128: 10,668 places of 66 KB with chunks
+    // of 49, 64 with chunks of 98)
+    const int64_t tile_rows = plan->max_q_rows * pack, row_bytes = d * sizeof(float) + sizeof(float2);
+    int64_t shares, n_long, split_tiles, all;
+    for (;; chunk *= 2) {
+        shares = longest > chunk ? (longest + chunk - 1) / chunk : 1;
+        n_long = plan->n_qb;  // query blocks whose lists are longer than a chunk
+        if (!d_sel) {
+            const int4* seq = std::partition_point(plan->by_length, plan->by_length + plan->n_by_length,
+                                                   [&](const int4& s) { return s.x > chunk; });
+            n_long = seq == plan->by_length ? 0 : seq[-1].y;
+        }
+        split_tiles = n_long * per_block;
+        all = split_tiles * shares;
+        if (shares == 1 || all * tile_rows * row_bytes <= kMaxPartBytes) break;
     }
-    const int64_t split_tiles = n_long * per_block, row_bytes = d * sizeof(float) + sizeof(float2);
-    const int64_t all = split_tiles * shares, filled = all < work / chunk + split_tiles ? all : work / chunk + split_tiles;
-    const int64_t tile_rows = plan->max_q_rows * pack;
-    const bool split = last - chunk >= kMinSaved + filled * tile_rows / kJoinRows &&
-                       (tiles <= slots / 2 || all * tile_rows * row_bytes <= kMaxPartBytes);
+    const int64_t filled = all < work / chunk + split_tiles ? all : work / chunk + split_tiles;
+    const bool split = last - chunk >= kMinSaved + filled * tile_rows / kJoinRows;
     CUtensorMap qm, km, vm;
     S3DSP_TRY(encode_q(&qm, q, plan->n_q, heads, d, q_stride, pack, f16, error, error_capacity));
     // a plan without key rows lists nothing: its maps are never read through

@@ -994,3 +994,19 @@ def test_block_select_holds_at_most_512_mb_of_scores(ctx, lens, klens, heads, to
             want = score.topk(top, dim=-1).indices.sort(dim=-1).values
         assert torch.equal(sel[b0:b0 + nb].long(), want)
         q0, k0, b0 = q0 + m, k0 + mk, b0 + nb
+
+
+@pytest.mark.parametrize("n,long,short,d", [(84, 6213, 50, 128), (149, 6000, 50, 128), (90, 5000, 40, 64)])
+def test_attention_partial_sums_are_bounded(ctx, n, long, short, d):
+    """One long list among many that are a little longer than a chunk: at most 256 MB of partial sums."""
+    lens, klens = [128] * n, [64 * short] * 20 + [64 * long] + [64 * short] * (n - 21)
+    q = randn((sum(lens), d), 1, torch.bfloat16)
+    k, v = randn((sum(klens), d), 2, torch.bfloat16), randn((sum(klens), d), 3, torch.bfloat16)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    out = torch.full_like(q, 7.0)
+    ctx.check()
+    used = s3dsp.memory_stats(0, reset_high=True)["used"]
+    ctx.block_attention(plan, q, k, v, 1, 1, out)
+    ctx.check()
+    assert s3dsp.memory_stats(0)["used_high"] - used <= 1 << 28
+    check(out, q, k, v, lens, klens, 1, 1, d ** -0.5)
