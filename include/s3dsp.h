@@ -431,7 +431,8 @@ S3DSP_API s3d_status s3dsp_qk_norm_rope(s3dsp_context *ctx, const void *q, int64
  * context's stream (not inside a stream capture; calls that use the plan may
  * be captured). Other contexts of the device may use the plan once that
  * stream has passed the call. Freed by s3dsp_attn_plan_free, in order of the
- * stream of the context it is given. */
+ * stream of the context it is given (NULL, when that context is gone: of the
+ * default stream). */
 S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context *ctx, const int64_t *h_q_offsets,
                                             const int64_t *h_k_offsets, int64_t n_seq, s3dsp_attn_plan **out,
                                             char *error, uint64_t error_capacity);

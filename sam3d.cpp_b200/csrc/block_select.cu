@@ -580,10 +580,8 @@ extern "C" S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context* ctx, const
 
 extern "C" S3DSP_API void s3dsp_attn_plan_free(s3dsp_context* ctx, s3dsp_attn_plan* plan) {
     if (!plan) return;
-    if (ctx) {
-        cudaSetDevice(ctx->device);
-        cudaFreeAsync(plan->mem, ctx->stream);
-    }
+    cudaSetDevice(plan->device);
+    cudaFreeAsync(plan->mem, ctx ? ctx->stream : nullptr);
     ::operator delete(plan->by_length);
     ::operator delete(plan->group_first);
     delete plan;

@@ -1010,3 +1010,17 @@ def test_attention_partial_sums_are_bounded(ctx, n, long, short, d):
     ctx.check()
     assert s3dsp.memory_stats(0)["used_high"] - used <= 1 << 28
     check(out, q, k, v, lens, klens, 1, 1, d ** -0.5)
+
+
+def test_a_plan_outlives_its_context():
+    """Freed after its context: the block tables go back to the pool."""
+    c = s3dsp.Context(0)
+    c.check()
+    torch.cuda.synchronize()
+    used = s3dsp.memory_stats(0)["used"]
+    plan = c.attn_plan(offsets([5000] * 2000))
+    assert s3dsp.memory_stats(0)["used"] >= used + plan.q_blocks * 32 + plan.k_blocks * 8
+    c.close()
+    plan.free()
+    torch.cuda.synchronize()
+    assert s3dsp.memory_stats(0)["used"] <= used
