@@ -196,8 +196,9 @@ class CoarseAttention:
         h + out( attention( R(pos) norm(q), R(pos) norm(k), v ) ),  q, k, v = Linears of LayerNorm(h)
 
     in BF16 with f32 rows h in and out: the per-head norms and the rotation by
-    the voxel position in one pass (s3dsp_qk_norm_rope; a third of a head's
-    pairs for each of x, y, z), attention over every coarse row of the row's
+    the voxel position in one pass (s3dsp_qk_norm_rope; `axis_pairs` of a head's
+    pairs for x, y, z, a third for each when None; (): no rotation, for rows
+    that carry their position already, as after the generator's APE), attention over every coarse row of the row's
     object, or with `top` > 0 over the `top` blocks of 64 rows that
     s3dsp_block_select picks for each 128 query rows and head (the block of the
     rows themselves among them). The objects of a batch are its sequences.
@@ -207,12 +208,13 @@ class CoarseAttention:
     has written, and buffers freed on return are reused in that order. Results
     are that stream's; a caller on another one waits for it."""
 
-    def __init__(self, s3dsp, ctx, params: dict, heads: int, device, top: int = 0, theta: float = 10000.0):
+    def __init__(self, s3dsp, ctx, params: dict, heads: int, device, top: int = 0, theta: float = 10000.0,
+                 axis_pairs=None):
         import torch
         self.s, self.ctx, self.torch, self.dev = s3dsp, ctx, torch, device
         self.c, self.heads, self.top, self.theta = params["out"]["w"].shape[0], heads, top, theta
         self.stream = ctx.torch_stream()
-        self.pairs = [self.c // heads // 6] * 3
+        self.pairs = [self.c // heads // 6] * 3 if axis_pairs is None else list(axis_pairs)
 
         def dev(a):
             return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).to(device)

@@ -1024,3 +1024,27 @@ def test_a_plan_outlives_its_context():
     plan.free()
     torch.cuda.synchronize()
     assert s3dsp.memory_stats(0)["used"] <= used
+
+
+@pytest.mark.parametrize("pairs", [(), (5, 0, 20), None])
+def test_coarse_attention_axis_pairs(ctx, pairs):
+    """The layer without a rotation (rows that carry their position already), with pairs dealt otherwise, and as it is
+    by default: q and k against the norm's definition and the rotation's."""
+    device = torch.device("cuda", 0)
+    coords = torch.from_numpy(np.ascontiguousarray(workloads.ellipsoid_shell(24, 1))).cuda()
+    heads, c = 4, 256
+    d = c // heads
+    params = slat.attention_params(c, heads)
+    layer = slat.CoarseAttention(s3dsp, ctx, params, heads, device, axis_pairs=pairs)
+    tb = slat.SlatTablesDev(s3dsp, ctx, coords, torch)
+    tables, t = layer.tables(tb), {}
+    layer.forward(tables, randn((tb.nc, c), 1), taps=t)
+    ctx.check()
+    for name, wk, rows in (("q", "q", slice(0, c)), ("k", "kv", slice(0, c))):
+        w = torch.from_numpy(params[wk]["w"][rows]).cuda().to(torch.bfloat16).double()
+        a = (t["x"].double() @ w.T + torch.from_numpy(params[wk]["b"][rows]).cuda().double()).reshape(-1, heads, d)
+        a = a / (a.square().mean(-1, keepdim=True) + 1e-6).sqrt() * torch.from_numpy(params[name + "_gamma"]).cuda().double()
+        used = [d // 6] * 3 if pairs is None else list(pairs)
+        want = turned(a.reshape(-1, c), tables[0][:, 1:], heads, used, 1e4, False, False)[0]
+        gate(float((t[name].double() - want).norm() / want.norm()), 1e-2, name)
+    check(t["a"], t["q"], t["k"], t["v"], [tb.nc], [tb.nc], heads, heads, d ** -0.5)
