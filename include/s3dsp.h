@@ -396,8 +396,9 @@ S3DSP_API s3d_status s3dsp_window_attention(s3dsp_context *ctx, const float *qkv
  * pairs turn with position column 0, the next axis_pairs[1] with column 1, ...;
  * the rest stay. Pair i of an axis with p pairs turns by pos * theta^(-i/p);
  * (a, b) -> (a cos - b sin, a sin + b cos). Angles are reduced to a turn in f64
- * (within |pos| 2^-50 for every int32 position), their remainder is f32. d_pos: device int32 rows with a stride of
- * pos_stride elements; voxel rows (batch, x, y, z) are d_coords + 1 with
+ * (within |pos| 2^-50 for every int32 position when theta >= 1), their
+ * remainder is f32. d_pos: device int32 rows with a stride of pos_stride
+ * elements; voxel rows (batch, x, y, z) are d_coords + 1 with
  * stride 4. d a multiple of 8 up to 256; any strides >= heads * d and element
  * alignment (16-byte aligned rows are read and written 16 bytes at a time).
  * y may be x with the same stride and type, and must not overlap it
@@ -429,8 +430,8 @@ S3DSP_API s3d_status s3dsp_qk_norm_rope(s3dsp_context *ctx, const void *q, int64
  * S3DSP_ATTN_Q_ROWS rows and key blocks of S3DSP_ATTN_K_ROWS, counted from
  * its own first row, the last ones shorter. Made from host memory on the
  * context's stream (not inside a stream capture; calls that use the plan may
- * be captured). Other contexts of the device may use the plan once that
- * stream has passed the call. Freed by s3dsp_attn_plan_free, in order of the
+ * be captured; keep the plan until their graphs are released). Other contexts
+ * of the device may use the plan once that stream has passed the call. Freed by s3dsp_attn_plan_free, in order of the
  * stream of the context it is given (NULL, when that context is gone: of the
  * default stream). */
 S3DSP_API s3d_status s3dsp_attn_plan_create(s3dsp_context *ctx, const int64_t *h_q_offsets,
@@ -446,7 +447,8 @@ S3DSP_API s3d_status s3dsp_attn_plan_info(const s3dsp_attn_plan *plan, int64_t *
  * block's k rows>: d_sel int32 [q blocks, heads, top], ascending indices
  * counted from the sequence's first key block, -1 behind them when the
  * sequence has fewer. Ties go to the lowest index, a NaN score is the lowest.
- * Means and scores are f64, so a list does not depend on the order of sums.
+ * Means and scores are f64, each summed in one fixed order, so a list repeats
+ * and equal blocks have equal scores.
  * keep_local != 0 (self attention plans only): the key blocks of the query
  * block's own rows come first. d a multiple of 8 up to 256, any strides; a
  * sequence with query rows has at most 28,000 key blocks. */

@@ -7,8 +7,8 @@
 //
 // A selection is whole numbers: two scores that differ by less than f32
 // rounding would swap blocks between two ways of adding the same rows, so the
-// sums, means and scores are f64 (exact sums of 16-bit rows, in practice). The
-// f64 work is 1 / (128 * 64) of the attention it steers.
+// sums, means and scores are f64 (exact sums of 16-bit rows, in practice), each
+// added in one fixed order, whatever the grid. The f64 work is 1 / (128 * 64) of the attention it steers.
 //
 //   block_mean_kernel   one pass over q and k (memory bound): a warp lane owns eight columns, eight
 //                       warps share the block's rows, f64 sums joined in warp order
@@ -17,10 +17,12 @@
 //                       64-bit keys whose unsigned order is the scores'
 //   top_warp_kernel     one warp per (query block, head): the top-th largest key by bisection, the
 //                       keys' upper halves in registers; the chosen indices in ascending order
-//   top_block_kernel    the same with one CTA per row and the keys in shared memory, for sequences
-//                       of more key blocks than a warp's registers take
+//   top_block_kernel    the same with one CTA per row and the keys in shared memory, for a batch with a
+//                       sequence of more key blocks than a warp's registers take (1,024): up to 64
+//                       counts over the keys, each with two barriers; 65,600 rows (1,025 key blocks) 365 us
+//                       against 140 for 65,500
 //
-// 65,500 rows, 16 heads of 64, bf16, lists of 32 (one B200): 142 us, of which the means 54 (268 MB
+// 65,500 rows, 16 heads of 64, bf16, lists of 32 (one B200): 141 us, of which the means 54 (268 MB
 // at 5.0 TB/s), the scores 55, the lists 30. Scores in f32 with an error bound, and f64 only where
 // the bound leaves a list in doubt: scores 37, lists 40, 135 us in all; at 28,000 and 1,900 rows
 // 70 and 27 us where this takes 66 and 25. Means with the 16-bit values taken to f64 by integer
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(128) top_warp_kernel(const ScoreParams p) {
             k[i] = is ? key64[c[i]] : 0ull;
         }
         unsigned long long a = (unsigned long long)lo << 32;
-        unsigned long long z = up > 0xffffffffull ? ~0ull : ((unsigned long long)up << 32) - 1;  // no key is above z
+        unsigned long long z = up > 0xffffffffull ? ~0ull : ((unsigned long long)up << 32) - 1;  // fewer than top are above z
         // the largest threshold in [a, z] that `top` keys reach
         int at_a = n;
         while (a < z && at_a != p.top) {
