@@ -466,7 +466,9 @@ S3DSP_API s3d_status s3dsp_block_select(s3dsp_context *ctx, const s3dsp_attn_pla
  * are. dtype S3DSP_BF16 or S3DSP_F16 for q, k, v and out; scores, softmax
  * statistics and sums in f32, the weights exp(s - max) rounded to dtype for
  * the product with v (tcgen05 MMAs; f16 keeps 11 bits of a weight down to
- * 2^-21 of the row's largest, and none below 2^-32). d 64 or 128; scale > 0 and finite;
+ * 2^-21 of the row's largest, and none below 2^-32; where |scale * score|
+ * passes 2^22, neighbouring f32 scores are about a power of two apart, and
+ * weights below the largest are as rough). d 64 or 128; scale > 0 and finite;
  * pointers 16-byte aligned, row strides multiples of 8 elements. out must not
  * overlap the inputs. */
 S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context *ctx, const s3dsp_attn_plan *plan, const void *q,

@@ -38,6 +38,7 @@
 //            exponentials busy 62 % of the cycles each
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "tc_common.cuh"
 
@@ -59,6 +60,16 @@ constexpr float kSlack = 8.f;
 // single large one came out wrong by up to their whole sum.
 template <bool kF16>
 constexpr float kShift = kF16 ? 7.f : -kSlack;
+// A score's weight is 2^(slope s + bias), one FMA: slope = c, and bias = kShift - c m
+// rounded once for the row, so that a row's reference is its bias, and what it has summed up is
+// rescaled by the difference of two. Past this value of c |m|, where neighbouring f32 scores are about
+// a power of two apart, the rounding of c m would decide a weight: the slope is c's power of two
+// (or less, where slope m ends), with which slope m is exact.
+constexpr float kFar = 1 << 23;
+template <bool kF16>
+__device__ __forceinline__ float weight_shift(float m, float c) {
+    return fabsf(m) * c > kFar ? 0.f : kShift<kF16>;
+}
 constexpr int kMinChunk = 4;    // key blocks of a chunk of a split list, at least
 constexpr int kMaxChunks = 128;
 constexpr int kMinSaved = 10;   // key blocks that a split has to take off the longest list
@@ -461,8 +472,19 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
         const int row = threadIdx.x;
         const uint32_t t0 = tmem + ((uint32_t)(32 * warp) << 16);
         const bool live = 32 * warp < q_rows;  // a warp without rows only keeps the barriers' counts
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, slope = p.c, bias = 0.f;
         bool ok = true;
+        // m as the row's maximum (a maximum of -inf weighs its scores of -inf by 0, one of inf or NaN makes the row NaN)
+        auto refer = [&](float to) {
+            m = to;
+            slope = p.c;
+            bias = m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m + kShift<kF16>);
+            if (fabsf(m) * p.c > kFar && fabsf(m) < INFINITY) {  // without kShift
+                auto power = [](float v) { return __uint_as_float(__float_as_uint(v) & 0x7f800000u); };
+                slope = fminf(power(p.c), power(0x1p126f / fabsf(m)));
+                bias = -m * slope;
+            }
+        };
         auto wait = [&](uint32_t bar, uint32_t parity) {
             return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status)) != 0;
         };
@@ -527,12 +549,10 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
 #pragma unroll
                 for (int x = 0; x < kK; x += 2)
                     mx[(x / 2) & 3] = max3(mx[(x / 2) & 3], __uint_as_float(s[x / 32][x % 32]), __uint_as_float(s[x / 32][x % 32 + 1]));
-                m = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+                refer(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
             }
             F2 sum[2];
             for (int attempt = 0;; ++attempt) {
-                // (an infinite maximum makes its row NaN, as inf - inf does)
-                const F2 bias = both(m == -INFINITY ? 0.f : fmaf(-m, p.c, m - m + kShift<kF16>));
                 float mx[2] = {m, m};
                 sum[0] = sum[1] = both(0.f);
 #pragma unroll
@@ -542,7 +562,7 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
                     for (int x = 0; x < 16; ++x) {
                         const F2 sc = {__uint_as_float(s[half][2 * x]), __uint_as_float(s[half][2 * x + 1])};
                         mx[x & 1] = max3(mx[x & 1], sc.x, sc.y);
-                        F2 v = fma2v(sc, both(p.c), bias);
+                        F2 v = fma2v(sc, both(slope), both(bias));
                         v = F2{exp2_hw(v.x), exp2_hw(v.y)};
                         sum[x & 1] = add2v(sum[x & 1], v);
                         w[x] = pack2<kF16>(v.x, v.y);
@@ -553,8 +573,13 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
                 // a NaN maximum counts as grown, and stays
                 const bool grown = !((mt - m) * p.c <= kSlack) && !(mt == -INFINITY);
                 if (attempt > 0 || !__any_sync(0xffffffffu, grown)) break;
-                const float to = grown ? mt : m;
-                const float alpha = grown ? exp2_hw((m - to) * p.c) : 1.f;
+                float alpha = 1.f;
+                if (grown) {
+                    const float from = m, before = bias;
+                    refer(mt);
+                    const float was = weight_shift<kF16>(from, p.c), is = weight_shift<kF16>(m, p.c);
+                    alpha = exp2_hw(was != 0.f && is != 0.f ? bias - before : (from - m) * p.c + (is - was));
+                }
                 if (j > 0) {
                     ok = wait(o_done + 8 * ob.slot, ob.parity);
                     if (!ok) break;
@@ -569,7 +594,6 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
                     }
                 }
                 l *= alpha;
-                m = to;
             }
             if (!ok) break;
             const F2 total = add2v(sum[0], sum[1]);
@@ -592,7 +616,11 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
             const int64_t out_row = q_row0 + row / p.pack;
             const int head = h + row % p.pack;
             const int64_t part = (int64_t)blockIdx.x * p.tile_rows + row;
-            if (split && row < q_rows) p.part_ml[part] = make_float2(m, l);
+            // a chunk's sums are handed on against the maximum itself, with 2^kShift
+            float exact = 1.f;
+            if (split && fabsf(m) < INFINITY)
+                exact = exp2_hw(kShift<kF16> - (slope == p.c ? fmaf(m, p.c, bias) : 0.f));
+            if (split && row < q_rows) p.part_ml[part] = make_float2(m, l * exact);
             uint16_t* dst = static_cast<uint16_t*>(p.out) + out_row * p.out_stride + (int64_t)head * D;
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -608,8 +636,8 @@ __global__ void __launch_bounds__(Cfg<D>::kRegThreads, 2)
                     float4* d4 = reinterpret_cast<float4*>(p.part_o + part * D + c0);
 #pragma unroll
                     for (int y = 0; y < 8; ++y)
-                        d4[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]),
-                                            __uint_as_float(o[4 * y + 2]), __uint_as_float(o[4 * y + 3]));
+                        d4[y] = make_float4(__uint_as_float(o[4 * y]) * exact, __uint_as_float(o[4 * y + 1]) * exact,
+                                            __uint_as_float(o[4 * y + 2]) * exact, __uint_as_float(o[4 * y + 3]) * exact);
                     continue;
                 }
                 uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
@@ -903,7 +931,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
         p.tiles = (int)split_tiles;
         p.split_ctas = (int)all;
     }
-    p.c = scale * 1.4426950408889634f;
+    p.c = std::min(scale * 1.4426950408889634f, std::numeric_limits<float>::max());
     p.q = q;
     p.q_stride = q_stride;
     p.out = out;

@@ -1048,3 +1048,67 @@ def test_coarse_attention_axis_pairs(ctx, pairs):
         want = turned(a.reshape(-1, c), tables[0][:, 1:], heads, used, 1e4, False, False)[0]
         gate(float((t[name].double() - want).norm() / want.norm()), 1e-2, name)
     check(t["a"], t["q"], t["k"], t["v"], [tb.nc], [tb.nc], heads, heads, d ** -0.5)
+
+
+# ---------------------------------------------------------------------------------------------------
+# scores far from 0: a softmax sees their differences
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("offset", ["all", "later", "below", "below at first", "rows"])
+@pytest.mark.parametrize("power", [10, 13, 16, 20, 30])
+@pytest.mark.parametrize("lens,klens,heads,kv,d", [
+    ([130], [1500], 2, 1, 64), ([130], [1500], 2, 1, 128),                # split lists
+    ([700], [1500], 32, 8, 64), ([700], [1500], 32, 8, 128), ([5, 100], [40, 200], 2, 2, 64),
+])
+def test_attention_of_far_scores(ctx, lens, klens, heads, kv, d, power, offset, dt):
+    """Scores (offset + x) / 2, exact in f32: an offset of 2^power to all keys, to those after the first 100, below 0,
+    below 0 for the first 100 only, or of another size for each row; x whole numbers that grow along the keys. Each
+    score's exponential is then off by less than 2^-18 (the rounding of an exponent up to 60, and ex2's 2^-22)."""
+    if power == 30 and (offset != "below at first" or min(klens) <= 100):
+        return  # a row whose scores are all 2^30 + x, which is no f32 (31 bits)
+    nq, nk = sum(lens), sum(klens)
+    q = torch.zeros((nq, heads, d), dtype=DT[dt], device="cuda")
+    k = torch.zeros((nk, kv, d), dtype=DT[dt], device="cuda")
+    v = randn((nk, kv * d), 3, DT[dt])
+    place = torch.cat([torch.arange(m, device="cuda") for m in klens])
+    x = (place * 60.0 / max(klens) + 12.0 * torch.rand(nk, generator=torch.Generator("cuda").manual_seed(1), device="cuda")).round()
+    q[:, :, 1], k[:, :, 1] = 1.0, x[:, None]
+    a, b = 2.0 ** (power // 2), 2.0 ** (power - power // 2)
+    q[:, :, 5] = a
+    if offset == "rows":
+        q[:, :, 5] *= 2.0 ** -(torch.arange(nq, device="cuda") % 8)[:, None]
+    sign = {"all": (1, 1), "later": (0, 1), "below": (-1, -1), "below at first": (-1, 0), "rows": (1, 1)}[offset]
+    k[:, :, 5] = torch.where(place < 100, sign[0] * b, sign[1] * b)[:, None]
+    q, k = q.flatten(1), k.flatten(1)
+    plan = ctx.attn_plan(offsets(lens), offsets(klens))
+    out = torch.full_like(q, 7.0)
+    ctx.block_attention(plan, q, k, v, heads, kv, out, scale=0.5)
+    ctx.check()
+    want, (mass, _) = attention(q, k, v, lens, klens, heads, kv, 0.5)
+    u = unit(DT[dt])
+    tol = mass.flatten(1) * (u + 2.0 ** -17 + 16 * F32)
+    if dt == "f16":
+        tol = tol + 2.0 ** -32 * float(v.abs().max()) * max(klens)
+    within(out, want, tol, u)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("scale", [1.0, 0.3, 1e-3])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_far_apart_scores(ctx, d, scale, dt):
+    """Exact scores up to 2^36 apart by 2^28 and more: each row is the value of its largest key, whatever its place."""
+    n = 300
+    q = torch.full((n, d), 2.0 ** 15, dtype=DT[dt], device="cuda")
+    q[::3] *= -1.0
+    order = torch.from_numpy(np.random.default_rng(d).permutation(n).astype(np.float32)).cuda() - 100.0
+    order = torch.where(order.abs() > 120, order.sign() * 119, order)  # whole numbers that both types keep, with ties
+    order[17], order[211] = 127.0, -126.0
+    k = (order * 128.0).to(DT[dt])[:, None].expand(n, d).contiguous()
+    v = randn((n, d), 3, DT[dt])
+    plan = ctx.attn_plan([0, n])
+    out = torch.empty_like(q)
+    ctx.block_attention(plan, q, k, v, 1, 1, out, scale=scale)
+    ctx.check()
+    best = torch.full((n,), 17, device="cuda")
+    best[::3] = 211
+    assert torch.equal(out, v[best])
