@@ -29,12 +29,12 @@
 // and their V rows by zeros in shared memory, whatever they hold.
 //
 // What bounds it (one B200, dense, 4,096 x 4,096 rows, 128 x 64 tiles):
-//   d = 64   148 heads, 823 us, 772 TFLOP/s (0.45 of the measured bf16 peak). The softmax warps: 64
+//   d = 64   148 heads, 827 us, 768 TFLOP/s (0.45 of the measured bf16 peak). The softmax warps: 64
 //            exponentials a row and tile at 16 a cycle and SM are 512 cycles, a tile takes about 690
 //            (1.7 GHz under this load); MMAs and barriers alone 540 us. A part of the exponentials on
 //            the FMA pipe (a polynomial): 851 us with one in eight, 894 with two. Two threads per row, or
 //            two groups of softmax warps per CTA: 909, 896. One warp for all MMAs: 868.
-//   d = 128  74 heads, 518 us, 1,227 TFLOP/s (0.73): MMAs and barriers alone 456 us; tensor pipe and
+//   d = 128  74 heads, 516 us, 1,232 TFLOP/s (0.73): MMAs and barriers alone 456 us; tensor pipe and
 //            exponentials busy 62 % of the cycles each
 #include <algorithm>
 #include <cmath>
@@ -859,10 +859,10 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // the split has to save the time of kMinSaved blocks, and of one more per
     // kJoinRows rows of partial sums: a block takes a CTA about 0.7 us (d = 64), the
     // joining kernel about 6 and its traffic. Without and with the split: 8 rows
-    // over 92k keys, 4 key heads, 527 and 41 us; 2,000 rows over 20,000, 4 heads, 203
-    // and 87; 1,024 over 2,048, 8 heads, 29 and 25; 1,024 over 1,024, 18 and 22 (not
+    // over 92k keys, 4 key heads, 527 and 42 us; 2,000 rows over 20,000, 4 heads, 203
+    // and 91; 1,024 over 2,048, 8 heads, 29 and 25; 1,024 over 1,024, 18 and 22 (not
     // split); eight sequences of 1,000 rows, one over 20,000 keys, the others over
-    // 100, 257 and 95. Sharing only the tiles of a last, half empty wave was measured
+    // 100, 257 and 97. Sharing only the tiles of a last, half empty wave was measured
     // too, 720 tiles of 119 blocks: 304 us against 290. A CTA alone on an SM runs
     // 1.2x as fast as one of two.
     const int64_t tiles = (int64_t)plan->n_qb * (heads / pack), slots = 2 * (int64_t)ctx->sm_count;
@@ -885,7 +885,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     // Every split tile has `shares` places, as many as the longest list takes. Where many lists are little
     // longer than a chunk most of these stay empty: chunks are made longer until the places fit
     // kMaxPartBytes (one list of 6,213 blocks beside 83 of 50, d = 128: 10,668 places of 66 KB with chunks
-    // of 49 and 219 us, 64 with chunks of 98 and 85 us)
+    // of 49 and 219 us, 64 with chunks of 98 and 89 us)
     const int64_t tile_rows = plan->max_q_rows * pack, row_bytes = d * sizeof(float) + sizeof(float2);
     int64_t shares, n_long, split_tiles, all;
     for (;; chunk *= 2) {

@@ -19,7 +19,7 @@
 //                       keys' upper halves in registers; the chosen indices in ascending order
 //   top_block_kernel    the same with one CTA per row and the keys in shared memory, for a batch with a
 //                       sequence of more key blocks than a warp's registers take (1,024): up to 64
-//                       counts over the keys, each with two barriers; 65,600 rows (1,025 key blocks) 365 us
+//                       counts over the keys, each with two barriers; 65,600 rows (1,025 key blocks) 367 us
 //                       against 140 for 65,500
 //
 // 65,500 rows, 16 heads of 64, bf16, lists of 32 (one B200): 141 us, of which the means 54 (268 MB

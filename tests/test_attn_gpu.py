@@ -1112,3 +1112,31 @@ def test_attention_of_far_apart_scores(ctx, d, scale, dt):
     best = torch.full((n,), 17, device="cuda")
     best[::3] = 211
     assert torch.equal(out, v[best])
+
+
+def test_coarse_attention_in_a_graph():
+    """The layer captured on its context's stream and replayed, on new rows, beside an eager call."""
+    device = torch.device("cuda", 0)
+    stream = torch.cuda.Stream()
+    c = s3dsp.Context(0, stream=stream.cuda_stream, flags=s3dsp.CONTEXT_DEFERRED_CHECKS)
+    width = 256
+    layer = slat.CoarseAttention(s3dsp, c, slat.attention_params(width, 4), 4, device, top=3)
+    coords = np.concatenate([workloads.ellipsoid_shell(24, b, batch=b) for b in range(2)])
+    with torch.cuda.stream(stream):
+        tb = slat.SlatTablesDev(s3dsp, c, torch.from_numpy(np.ascontiguousarray(coords)).cuda(), torch)
+        tables = layer.tables(tb)
+        h = [randn((tb.nc, width), seed) for seed in (1, 2, 3)]
+        want = [layer.forward(tables, x).clone() for x in h]
+        held = h[0].clone()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = layer.forward(tables, held)
+    for x, w in zip(h, want):
+        with torch.cuda.stream(stream):
+            held.copy_(x)
+            graph.replay()
+            eager = layer.forward(tables, h[0])
+        stream.synchronize()
+        assert torch.equal(y, w) and torch.equal(eager, want[0])
+    c.check()
