@@ -211,7 +211,7 @@ s3d_status check_status(s3dsp_context* ctx, char* error, uint64_t error_capacity
         return fail(error, error_capacity, S3D_INTERNAL_ERROR, "coordinate hash probe bound exceeded");
     if (st[0] & kErrRowRange)
         return fail(error, error_capacity, S3D_INVALID_ARGUMENT,
-                    "a row index passed in (upsample / composition rows) is outside its input table");
+                    "a row index passed in (upsample / composition rows), or a listed key block, is outside its table");
     if (st[0] & kErrPipelineTimeout)
         return fail(error, error_capacity, S3D_INTERNAL_ERROR,
                     "a device pipeline wait timed out (kernel aborted)");

@@ -1140,3 +1140,12 @@ def test_coarse_attention_in_a_graph():
         stream.synchronize()
         assert torch.equal(y, w) and torch.equal(eager, want[0])
     c.check()
+
+
+def test_the_report_of_an_absent_block_names_it(ctx):
+    q, k, v = (randn((128, 64), s, torch.bfloat16) for s in (1, 2, 3))
+    plan = ctx.attn_plan([0, 128])
+    ctx.block_attention(plan, q, k, v, 1, 1, torch.empty_like(q),
+                        sel=torch.tensor([[[0, 2]]], dtype=torch.int32, device="cuda"))
+    with pytest.raises(s3dsp.S3dError, match="listed key block"):
+        ctx.check()
