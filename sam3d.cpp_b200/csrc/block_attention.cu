@@ -918,7 +918,7 @@ extern "C" S3DSP_API s3d_status s3dsp_block_attention(s3dsp_context* ctx, const 
     p.n_qb = plan->n_qb;
     p.tile_rows = (int)tile_rows;
     // Where the lists' lengths differ, the longest start first, with all their heads, so that short ones
-    // fill the end: objects of 15,159, 4,211, 8,190 and 2,777 rows, 16 heads, 1,665 us against 1,800 in the
+    // fill the end: objects of 15,159, 4,211, 8,190 and 2,777 rows, 16 heads, 1,667 us against 1,800 in the
     // sequences' order, head by head, and 1,775 with the longest of each head first. Equal lengths stay in
     // their order, which reads a head's rows close together (forty objects of 300: 63 against 65).
     if (!d_sel && (split || 4 * (int64_t)longest * plan->n_qb > 5 * plan->sum_kb)) p.order = plan->order;

@@ -206,7 +206,8 @@ class CoarseAttention:
     Torch's part (allocations, the count of each object's rows) runs on the
     context's stream too, whichever is current: torch reads what the library
     has written, and buffers freed on return are reused in that order. Results
-    are that stream's; a caller on another one waits for it."""
+    are that stream's; a caller on another one waits for it, and records its own
+    stream on what it drops (Tensor.record_stream)."""
 
     def __init__(self, s3dsp, ctx, params: dict, heads: int, device, top: int = 0, theta: float = 10000.0,
                  axis_pairs=None):
